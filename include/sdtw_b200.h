@@ -312,6 +312,122 @@ int sdtw_grad_sqeuclid_f64(const double *G, const double *x, const double *y, do
 int sdtw_forward_noalloc_f32(const float *D, float *score, float *out, int B, int N, int M, float gamma,
                              float bandwidth, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Sequence operators: layers of a model whose output series the loss compares.
+ * No counterpart in the reference package.  Series are (batch, length, dim),
+ * features last and contiguous, with element strides for the batch and the
+ * time step; a tensor listed as contiguous has none.  `dtype` is the type of
+ * the series (SDTW_F32, SDTW_F16, SDTW_BF16); parameters, recurrent states and
+ * parameter gradients are float32, and so is all arithmetic.  lengths (batch,)
+ * int64 on the device, or NULL: the valid steps of each series, clamped to
+ * [0, length]; steps beyond are never read into a result, their outputs and
+ * gradients are 0.  Optional pointers may be NULL.  The blocks are read
+ * during the call only. */
+#define SDTW_F32 0
+#define SDTW_F16 1
+#define SDTW_BF16 2
+
+/* Layer norm over the features of each row:
+ *   y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps),
+ * var the mean of (x - mean)^2.  The backward takes the forward's mean and rstd
+ * and writes dx and the sums over the rows dweight, dbias (each optional). */
+typedef struct {
+    int dtype, dim;
+    long long rows;
+    float eps;
+    const void *x;      /* (rows, dim) */
+    long long x_stride; /* elements between rows */
+    const float *weight, *bias; /* (dim,), optional (1 and 0) */
+    void *y;            /* forward: (rows, dim) contiguous */
+    float *mean, *rstd; /* (rows,): forward outputs (both or neither), backward inputs */
+    const void *dy;     /* backward: (rows, dim) */
+    long long dy_stride;
+    void *dx;           /* backward: (rows, dim) contiguous, optional */
+    float *dweight, *dbias; /* backward: (dim,), optional */
+    void *workspace;    /* backward: sdtw_layer_norm_workspace_bytes */
+    size_t workspace_bytes;
+} sdtw_layer_norm_args;
+size_t sdtw_layer_norm_workspace_bytes(long long rows, int dim);
+int sdtw_layer_norm_forward(const sdtw_layer_norm_args *args, void *stream);
+int sdtw_layer_norm_backward(const sdtw_layer_norm_args *args, void *stream);
+
+/* Causal convolution of each feature over time, 1 <= width <= 8:
+ *   v[t] = bias + sum_k weight[:, k] * s[t + k],   y = v, or v * sigmoid(v) with silu,
+ * where s is state_in (the width - 1 inputs before the series; NULL = zeros)
+ * followed by x.  state_out, if given, gets the last width - 1 inputs of s (of
+ * each series' own length), so that a later call goes on from there.
+ * sdtw_conv_step is the length-1 form for a running state: state_in
+ * and state_out may be the same tensor, and lengths is not used.
+ * The backward writes dx, dstate_in, dweight and dbias (each optional) from dy
+ * and dstate_out (optional). */
+typedef struct {
+    int dtype, batch, length, dim, width, silu;
+    const void *x;      /* (batch, length, dim) */
+    long long x_batch, x_time;
+    const float *weight; /* (dim, width) contiguous */
+    const float *bias;   /* (dim,), optional */
+    const long long *lengths;
+    const void *state_in; /* (batch, width - 1, dim), steps contiguous, optional */
+    long long state_in_batch;
+    void *state_out;    /* as state_in, optional */
+    long long state_out_batch;
+    void *y;            /* forward: contiguous */
+    const void *dy;     /* backward: (batch, length, dim) */
+    long long dy_batch, dy_time;
+    const void *dstate_out; /* backward: contiguous, optional */
+    void *dx;           /* backward: contiguous, optional */
+    void *dstate_in;    /* backward: contiguous, optional */
+    float *dweight, *dbias; /* backward: (dim, width), (dim,), optional */
+    void *workspace;    /* backward: sdtw_conv_workspace_bytes */
+    size_t workspace_bytes;
+} sdtw_conv_args;
+size_t sdtw_conv_workspace_bytes(int batch, int length, int dim, int width);
+int sdtw_conv_forward(const sdtw_conv_args *args, void *stream);
+int sdtw_conv_backward(const sdtw_conv_args *args, void *stream);
+int sdtw_conv_step(const sdtw_conv_args *args, void *stream);
+
+/* Selective scan: per feature d a state h of nstate values (1 .. 64),
+ *   dt = softplus(delta + delta_bias)   (or delta + delta_bias without softplus)
+ *   h[n] = exp(dt A[d, n]) h[n] + dt B[t, g, n] x[t, d]
+ *   y[t, d] = (sum_n C[t, g, n] h[n] + D[d] x[t, d]) * (z ? z sigmoid(z) : 1)
+ * with the group g = d / (dim / groups).  h starts as state_in (NULL = zeros);
+ * state_out, if given, gets h after each series' last valid step.  `saved`
+ * (sdtw_scan_saved_elems floats; NULL when no backward follows) keeps the state
+ * every 32 steps for the backward, which writes the gradients of every input
+ * (d* fields, each optional) from dy and dstate_out (optional).
+ * sdtw_scan_step is the length-1 form for a running state:
+ * state_in and state_out may be the same tensor, and lengths is not used. */
+typedef struct {
+    int dtype, batch, length, dim, groups, nstate, softplus;
+    const void *x, *delta, *z; /* (batch, length, dim); z optional */
+    long long x_batch, x_time, delta_batch, delta_time, z_batch, z_time;
+    const void *B, *C;         /* (batch, length, groups, nstate) */
+    long long B_batch, B_time, B_group, C_batch, C_time, C_group;
+    const float *A;            /* (dim, nstate) contiguous */
+    const float *D, *delta_bias; /* (dim,), optional */
+    const long long *lengths;
+    const float *state_in;     /* (batch, dim, nstate), each batch entry contiguous, optional */
+    long long state_in_batch;
+    float *state_out;          /* as state_in, optional */
+    long long state_out_batch;
+    float *saved;
+    void *y;                   /* forward: contiguous */
+    const void *dy;            /* backward: (batch, length, dim) */
+    long long dy_batch, dy_time;
+    const float *dstate_out;   /* backward: contiguous, optional */
+    void *dx, *ddelta, *dz;    /* backward: contiguous, optional */
+    void *dB, *dC;             /* backward: (batch, length, groups, nstate) contiguous, optional */
+    float *dA, *dD, *ddelta_bias; /* backward: contiguous, optional */
+    float *dstate_in;          /* backward: contiguous, optional */
+    void *workspace;           /* backward: sdtw_scan_workspace_bytes */
+    size_t workspace_bytes;
+} sdtw_scan_args;
+size_t sdtw_scan_saved_elems(int batch, int length, int dim, int nstate);
+size_t sdtw_scan_workspace_bytes(int batch, int length, int dim, int groups, int nstate);
+int sdtw_scan_forward(const sdtw_scan_args *args, void *stream);
+int sdtw_scan_backward(const sdtw_scan_args *args, void *stream);
+int sdtw_scan_step(const sdtw_scan_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@
 
 #include "../../include/sdtw_b200.h"
 #include "sdtw_kernels.h"
+#include "seq_kernels.h"
 
 // Device-side "some wait failed" flag, one per device that loads the library.
 __device__ int g_abort_flag;
@@ -1308,6 +1309,173 @@ int sdtw_forward_noalloc_f32(const float* D, float* score, float* out, int B, in
     w.status = status;
     w.diag = reinterpret_cast<volatile WaitDiag*>(status + 8);
     return run_forward(Dw, score, out, B, N, M, gamma, bandwidth, static_cast<uint64_t*>(base), st, false, &w);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- sequence operators
+namespace {
+
+int check_dtype(int dtype) {
+    if (dtype != SDTW_F32 && dtype != SDTW_F16 && dtype != SDTW_BF16)
+        return fail(SDTW_ERR_INVALID_ARGUMENT, "dtype must be SDTW_F32, SDTW_F16 or SDTW_BF16");
+    return SDTW_OK;
+}
+
+int check_series(int dtype, int batch, int length, int dim) {
+    int rc;
+    if ((rc = check_dtype(dtype))) return rc;
+    if (batch <= 0 || length <= 0 || dim <= 0) return fail(SDTW_ERR_INVALID_ARGUMENT, "batch, length and dim must be > 0");
+    if (length >= (1 << 30) || dim >= (1 << 28)) return fail(SDTW_ERR_INVALID_ARGUMENT, "length or dim too large");
+    return SDTW_OK;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+    if (need && (!ws || have < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
+        return fail(SDTW_ERR_INVALID_ARGUMENT, "workspace missing, not 256-byte aligned or too small");
+    return SDTW_OK;
+}
+
+int null_pointer() { return fail(SDTW_ERR_INVALID_ARGUMENT, "null pointer"); }
+
+// No exception leaves the C interface.
+template <typename F>
+int guarded(F&& body) noexcept {
+    try {
+        return body();
+    } catch (...) {
+        return SDTW_ERR_CUDA;
+    }
+}
+
+template <typename F>
+int run_kernels(const char* name, int kernels, void* stream, F&& launch) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    {
+        KernelTimer kt(name, st, kernels);
+        e = launch(st);
+    }
+    return e == cudaSuccess ? SDTW_OK : cuda_fail(e, name);
+}
+
+int check_conv(const sdtw_conv_args* a) {
+    int rc;
+    if (!a) return null_pointer();
+    if ((rc = check_series(a->dtype, a->batch, a->length, a->dim))) return rc;
+    if (a->width < 1 || a->width > kConvMaxWidth) return fail(SDTW_ERR_INVALID_ARGUMENT, "width must be between 1 and 8");
+    return a->x && a->weight ? SDTW_OK : null_pointer();
+}
+
+int check_scan(const sdtw_scan_args* a) {
+    int rc;
+    if (!a) return null_pointer();
+    if ((rc = check_series(a->dtype, a->batch, a->length, a->dim))) return rc;
+    if (a->nstate < 1 || a->nstate > kScanMaxState) return fail(SDTW_ERR_INVALID_ARGUMENT, "nstate must be between 1 and 64");
+    if (a->groups < 1 || a->dim % a->groups) return fail(SDTW_ERR_INVALID_ARGUMENT, "groups must divide dim");
+    return a->x && a->delta && a->A && a->B && a->C ? SDTW_OK : null_pointer();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sdtw_layer_norm_workspace_bytes(long long rows, int dim) {
+    return rows <= 0 || dim <= 0 ? 0 : layer_norm_bwd_ws(rows, dim);
+}
+
+int sdtw_layer_norm_forward(const sdtw_layer_norm_args* a, void* stream) {
+    return guarded([&] {
+        if (!a) return null_pointer();
+        if (int rc = check_dtype(a->dtype)) return rc;
+        if (a->rows <= 0 || a->dim <= 0) return fail(SDTW_ERR_INVALID_ARGUMENT, "rows and dim must be > 0");
+        if (!(a->eps >= 0.f)) return fail(SDTW_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+        if (!a->x || !a->y || !a->mean != !a->rstd) return null_pointer();
+        return run_kernels("layer_norm_fwd", 1, stream, [&](cudaStream_t st) { return launch_layer_norm_fwd(*a, st); });
+    });
+}
+
+int sdtw_layer_norm_backward(const sdtw_layer_norm_args* a, void* stream) {
+    return guarded([&] {
+        if (!a) return null_pointer();
+        if (int rc = check_dtype(a->dtype)) return rc;
+        if (a->rows <= 0 || a->dim <= 0) return fail(SDTW_ERR_INVALID_ARGUMENT, "rows and dim must be > 0");
+        if (!a->x || !a->dy || !a->mean || !a->rstd) return null_pointer();
+        const bool par = a->dweight || a->dbias;
+        if (!a->dx && !par) return static_cast<int>(SDTW_OK);
+        if (int rc = check_workspace(a->workspace, a->workspace_bytes, par ? layer_norm_bwd_ws(a->rows, a->dim) : 0)) return rc;
+        return run_kernels("layer_norm_bwd", par ? 2 : 1, stream, [&](cudaStream_t st) { return launch_layer_norm_bwd(*a, st); });
+    });
+}
+
+size_t sdtw_conv_workspace_bytes(int batch, int length, int dim, int width) {
+    return batch <= 0 || length <= 0 || dim <= 0 || width <= 0 ? 0 : conv_bwd_ws(batch, length, dim, width);
+}
+
+int sdtw_conv_forward(const sdtw_conv_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_conv(a)) return rc;
+        if (!a->y) return null_pointer();
+        return run_kernels("conv_fwd", 1, stream, [&](cudaStream_t st) { return launch_conv_fwd(*a, st); });
+    });
+}
+
+int sdtw_conv_backward(const sdtw_conv_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_conv(a)) return rc;
+        if (!a->dy) return null_pointer();
+        const bool par = a->dweight || a->dbias;
+        if (int rc = check_workspace(a->workspace, a->workspace_bytes,
+                                     par ? conv_bwd_ws(a->batch, a->length, a->dim, a->width) : 0))
+            return rc;
+        return run_kernels("conv_bwd", 1 + (par ? 1 : 0) + (a->dstate_in && a->width > 1 ? 1 : 0), stream, [&](cudaStream_t st) { return launch_conv_bwd(*a, st); });
+    });
+}
+
+int sdtw_conv_step(const sdtw_conv_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_conv(a)) return rc;
+        if (a->length != 1) return fail(SDTW_ERR_INVALID_ARGUMENT, "a step has length 1");
+        if (!a->y || (a->width > 1 && (!a->state_in || !a->state_out))) return null_pointer();
+        return run_kernels("conv_step", 1, stream, [&](cudaStream_t st) { return launch_conv_step(*a, st); });
+    });
+}
+
+size_t sdtw_scan_saved_elems(int batch, int length, int dim, int nstate) {
+    return batch <= 0 || length <= 0 || dim <= 0 || nstate <= 0 ? 0 : scan_states(batch, length, dim, nstate);
+}
+
+size_t sdtw_scan_workspace_bytes(int batch, int length, int dim, int groups, int nstate) {
+    if (batch <= 0 || length <= 0 || dim <= 0 || groups <= 0 || nstate <= 0 || nstate > kScanMaxState || dim % groups) return 0;
+    return scan_bwd_ws(batch, length, dim, groups, nstate);
+}
+
+int sdtw_scan_forward(const sdtw_scan_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_scan(a)) return rc;
+        if (!a->y) return null_pointer();
+        return run_kernels("scan_fwd", 1, stream, [&](cudaStream_t st) { return launch_scan_fwd(*a, st); });
+    });
+}
+
+int sdtw_scan_backward(const sdtw_scan_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_scan(a)) return rc;
+        if (!a->dy || !a->saved) return null_pointer();
+        if (int rc = check_workspace(a->workspace, a->workspace_bytes,
+                                     scan_bwd_ws(a->batch, a->length, a->dim, a->groups, a->nstate)))
+            return rc;
+        return run_kernels("scan_bwd", 2, stream, [&](cudaStream_t st) { return launch_scan_bwd(*a, st); });
+    });
+}
+
+int sdtw_scan_step(const sdtw_scan_args* a, void* stream) {
+    return guarded([&] {
+        if (int rc = check_scan(a)) return rc;
+        if (a->length != 1) return fail(SDTW_ERR_INVALID_ARGUMENT, "a step has length 1");
+        if (!a->y || !a->state_in || !a->state_out) return null_pointer();
+        return run_kernels("scan_step", 1, stream, [&](cudaStream_t st) { return launch_scan_step(*a, st); });
+    });
 }
 
 }  // extern "C"

@@ -1,0 +1,434 @@
+// layer_norm.cu -- layer norm over the features of each row, and its gradient.
+//
+//   y  = xh w + b,  xh = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   dx = rstd (g - mean(g) - xh mean(g xh)),  g = dy w
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+//
+// Memory bound: a forward reads x and writes y once, a backward reads x and dy
+// and writes dx once.  A row stays in the registers of TPR threads (a warp up to
+// 1024 features, so that the row's sums are shuffles and no barrier), both
+// statistics come from the registers (the variance around the mean, not as a
+// difference of squares), and the threads walk over rows with the weights, and
+// in the backward the column sums, held in registers.  Column sums go to one
+// partial row per block and a second kernel adds the blocks in a fixed order, so
+// results do not change from call to call.
+#include <algorithm>
+
+#include "seq_device.cuh"
+#include "seq_kernels.h"
+
+namespace sdtw {
+namespace {
+
+struct LnP {
+    const void *x, *dy;
+    void *y, *dx;
+    const float *w, *b;
+    float *mean, *rstd, *part;
+    long long rows, xs, dys;
+    int dim;
+    float eps;
+    int want_dx, want_part;
+};
+
+// Sum over the TPR threads of a row (a warp, or the whole block).  `buf` holds
+// two slots per warp: consecutive sums alternate, so that one barrier each is enough.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float (*buf)[TPR / 32], int& turn) {
+    v = warp_sum(v);
+    if constexpr (TPR > 32) {
+        float* s = buf[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) v += s[i];
+    }
+    return v;
+}
+
+// Thread `tid` of a row holds the features (k TPR + tid) VEC .. + VEC, k < NV.
+template <typename T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_fwd_kernel(const LnP p) {
+    constexpr int RPB = TPR > 128 ? 1 : 128 / TPR;
+    __shared__ float buf[2][TPR / 32];
+    int turn = 0;
+    const int tid = threadIdx.x % TPR;
+    const float inv = 1.f / static_cast<float>(p.dim);
+    float w[NV * VEC], b[NV * VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int c = (k * TPR + tid) * VEC + e;
+            w[k * VEC + e] = c < p.dim && p.w ? __ldg(p.w + c) : 1.f;
+            b[k * VEC + e] = c < p.dim && p.b ? __ldg(p.b + c) : 0.f;
+        }
+    const long long step = static_cast<long long>(gridDim.x) * RPB;
+    Vec<T, VEC> raw[NV];
+    auto fetch = [&](long long r) {
+        const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * TPR + tid) * VEC;
+            if (c < p.dim)
+                raw[k].load(xr + c);
+            else
+                raw[k].zero();
+        }
+    };
+    long long r = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
+    if (r < p.rows) fetch(r);
+    for (; r < p.rows; r += step) {
+        float v[NV * VEC];
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) {
+            v[i] = raw[i / VEC].get(i % VEC);
+            s += v[i];
+        }
+        if (r + step < p.rows) fetch(r + step);  // the next row is on its way during this one's sums
+        const float mean = row_sum<TPR>(s, buf, turn) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float& u = v[k * VEC + e];
+                u = (k * TPR + tid) * VEC + e < p.dim ? u - mean : 0.f;
+                s = fmaf(u, u, s);
+            }
+        const float rstd = rsqrtf(row_sum<TPR>(s, buf, turn) * inv + p.eps);
+        T* yr = static_cast<T*>(p.y) + r * p.dim;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * TPR + tid) * VEC;
+            Vec<T, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                o.set(e, fmaf(v[k * VEC + e] * rstd, w[k * VEC + e], b[k * VEC + e]));
+            if (c < p.dim) o.store(yr + c);
+        }
+        if (tid == 0 && p.mean) {
+            p.mean[r] = mean;
+            p.rstd[r] = rstd;
+        }
+    }
+}
+
+template <typename T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_bwd_kernel(const LnP p) {
+    constexpr int RPB = TPR > 128 ? 1 : 128 / TPR;
+    __shared__ float buf[2][TPR / 32];
+    int turn = 0;
+    const int tid = threadIdx.x % TPR;
+    const float inv = 1.f / static_cast<float>(p.dim);
+    float w[NV * VEC], dw[NV * VEC], db[NV * VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int c = (k * TPR + tid) * VEC + e;
+            w[k * VEC + e] = c < p.dim && p.w ? __ldg(p.w + c) : 1.f;
+            dw[k * VEC + e] = db[k * VEC + e] = 0.f;
+        }
+    const long long step = static_cast<long long>(gridDim.x) * RPB;
+    Vec<T, VEC> rx[NV], rg[NV];
+    float mean = 0.f, rstd = 0.f;
+    auto fetch = [&](long long r) {
+        const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+        const T* gr = static_cast<const T*>(p.dy) + r * p.dys;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * TPR + tid) * VEC;
+            if (c < p.dim) {
+                rx[k].load(xr + c);
+                rg[k].load(gr + c);
+            } else {
+                rx[k].zero();
+                rg[k].zero();
+            }
+        }
+        mean = __ldg(p.mean + r);
+        rstd = __ldg(p.rstd + r);
+    };
+    long long r = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
+    if (r < p.rows) fetch(r);
+    for (; r < p.rows; r += step) {
+        float xh[NV * VEC], g[NV * VEC];
+        float s1 = 0.f, s2 = 0.f;
+        const float rs = rstd;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = k * VEC + e;
+                const bool in = (k * TPR + tid) * VEC + e < p.dim;
+                xh[i] = in ? (rx[k].get(e) - mean) * rs : 0.f;
+                const float d = rg[k].get(e);
+                dw[i] = fmaf(d, xh[i], dw[i]);
+                db[i] += d;
+                g[i] = d * w[i];
+                s1 += g[i];
+                s2 = fmaf(g[i], xh[i], s2);
+            }
+        if (r + step < p.rows) fetch(r + step);
+        if (!p.want_dx) continue;
+        s1 = row_sum<TPR>(s1, buf, turn) * inv;
+        s2 = row_sum<TPR>(s2, buf, turn) * inv;
+        T* dr = static_cast<T*>(p.dx) + r * p.dim;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * TPR + tid) * VEC;
+            Vec<T, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = k * VEC + e;
+                o.set(e, rs * (g[i] - s1 - xh[i] * s2));
+            }
+            if (c < p.dim) o.store(dr + c);
+        }
+    }
+    if (!p.want_part) return;
+    float* pw = p.part + static_cast<size_t>(blockIdx.x) * 2 * p.dim;
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) {
+            const int c = (i / VEC * TPR + tid) * VEC + i % VEC;
+            if (c < p.dim) {
+                pw[c] = dw[i];
+                pw[p.dim + c] = db[i];
+            }
+        }
+    } else {
+        __shared__ float acc[RPB][32 * VEC];
+#pragma unroll
+        for (int k = 0; k < 2 * NV; ++k) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                acc[threadIdx.x / TPR][tid * VEC + e] = k < NV ? dw[k % NV * VEC + e] : db[k % NV * VEC + e];
+            __syncthreads();
+            for (int j = threadIdx.x; j < TPR * VEC; j += 128) {
+                float s = 0.f;
+#pragma unroll
+                for (int q = 0; q < RPB; ++q) s += acc[q][j];
+                const int c = k % NV * TPR * VEC + j;
+                if (c < p.dim) pw[k / NV * p.dim + c] = s;
+            }
+        }
+    }
+}
+
+// Rows of more than 8192 features: the row is read again for every pass.
+constexpr int kLong = 512;
+template <typename T>
+__global__ void __launch_bounds__(kLong) ln_fwd_long_kernel(const LnP p) {
+    __shared__ float buf[2][kLong / 32];
+    int turn = 0;
+    const float inv = 1.f / static_cast<float>(p.dim);
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+        float s = 0.f;
+        for (int c = threadIdx.x; c < p.dim; c += kLong) s += to_f(xr[c]);
+        const float mean = row_sum<kLong>(s, buf, turn) * inv;
+        s = 0.f;
+        for (int c = threadIdx.x; c < p.dim; c += kLong) {
+            const float u = to_f(xr[c]) - mean;
+            s = fmaf(u, u, s);
+        }
+        const float rstd = rsqrtf(row_sum<kLong>(s, buf, turn) * inv + p.eps);
+        T* yr = static_cast<T*>(p.y) + r * p.dim;
+        for (int c = threadIdx.x; c < p.dim; c += kLong)
+            yr[c] = from_f<T>(fmaf((to_f(xr[c]) - mean) * rstd, p.w ? p.w[c] : 1.f, p.b ? p.b[c] : 0.f));
+        if (threadIdx.x == 0 && p.mean) {
+            p.mean[r] = mean;
+            p.rstd[r] = rstd;
+        }
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(kLong) ln_bwd_long_kernel(const LnP p) {
+    __shared__ float buf[2][kLong / 32];
+    int turn = 0;
+    const float inv = 1.f / static_cast<float>(p.dim);
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+        const T* gr = static_cast<const T*>(p.dy) + r * p.dys;
+        const float mean = p.mean[r], rs = p.rstd[r];
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < p.dim; c += kLong) {
+            const float g = to_f(gr[c]) * (p.w ? p.w[c] : 1.f);
+            s1 += g;
+            s2 = fmaf(g, (to_f(xr[c]) - mean) * rs, s2);
+        }
+        s1 = row_sum<kLong>(s1, buf, turn) * inv;
+        s2 = row_sum<kLong>(s2, buf, turn) * inv;
+        T* dr = static_cast<T*>(p.dx) + r * p.dim;
+        for (int c = threadIdx.x; c < p.dim; c += kLong) {
+            const float g = to_f(gr[c]) * (p.w ? p.w[c] : 1.f);
+            dr[c] = from_f<T>(rs * (g - s1 - (to_f(xr[c]) - mean) * rs * s2));
+        }
+    }
+}
+// Their column sums: block (x, y) adds every gridDim.y-th row of 256 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) ln_cols_kernel(const LnP p) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.dim) return;
+    float dw = 0.f, db = 0.f;
+    for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
+        const float d = to_f(static_cast<const T*>(p.dy)[r * p.dys + c]);
+        dw = fmaf(d, (to_f(static_cast<const T*>(p.x)[r * p.xs + c]) - p.mean[r]) * p.rstd[r], dw);
+        db += d;
+    }
+    float* pw = p.part + static_cast<size_t>(blockIdx.y) * 2 * p.dim;
+    pw[c] = dw;
+    pw[p.dim + c] = db;
+}
+
+// dweight, dbias = sums of the blocks' partial rows: 32 columns per block, 32
+// slices of the rows, added in a fixed order.
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int nblk, int dim, float* dw, float* db) {
+    __shared__ float acc[32][33];
+    pdl_wait();
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (c < 2 * dim)
+#pragma unroll 4
+        for (int i = threadIdx.y; i < nblk; i += 32) s += part[static_cast<size_t>(i) * 2 * dim + c];
+    acc[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    s = warp_sum(acc[threadIdx.x][threadIdx.y]);
+    const int o = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && o < 2 * dim) {
+        if (o < dim) {
+            if (dw) dw[o] = s;
+        } else if (db) {
+            db[o - dim] = s;
+        }
+    }
+}
+
+// Threads per row: a warp as long as its lanes hold at most 32 features each
+// (sums without barriers), then 4 warps; 16 warps have registers for 16 each,
+// and longer rows (0) are not held at all.
+int threads_per_row(int dim) { return dim <= 32 * 32 ? 32 : (dim <= 128 * 32 ? 128 : (dim <= 512 * 16 ? 512 : 0)); }
+
+// Blocks of the backward, each of which leaves a partial row of column sums: as
+// many as are resident (16 warps per SM), but two rows per warp at least.
+int bwd_blocks(long long rows, int dim) {
+    const int tpr = threads_per_row(dim);
+    if (tpr == 0) return static_cast<int>(std::min<long long>(rows, 64));
+    const long long rpb = tpr == 32 ? 4 : 1;
+    const long long cap = tpr == 512 ? 148 : 592;
+    return static_cast<int>(std::max<long long>(1, std::min(cap, (rows + 2 * rpb - 1) / (2 * rpb))));
+}
+
+template <typename T, int VEC, int NV, int TPR>
+void run_ln(const LnP& p, bool bwd, int blocks, cudaStream_t st) {
+    constexpr int threads = TPR > 128 ? TPR : 128;
+    if (bwd)
+        ln_bwd_kernel<T, VEC, NV, TPR><<<blocks, threads, 0, st>>>(p);
+    else
+        ln_fwd_kernel<T, VEC, NV, TPR><<<blocks, threads, 0, st>>>(p);
+}
+template <typename T, int VEC, int NV>
+void run_ln_t(const LnP& p, int tpr, bool bwd, int blocks, cudaStream_t st) {
+    if constexpr (VEC * NV <= 16)
+        if (tpr == 512) return run_ln<T, VEC, NV, 512>(p, bwd, blocks, st);
+    if (tpr == 128)
+        run_ln<T, VEC, NV, 128>(p, bwd, blocks, st);
+    else
+        run_ln<T, VEC, NV, 32>(p, bwd, blocks, st);
+}
+
+template <typename T>
+cudaError_t run_ln_all(const LnP& p, bool bwd, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const int tpr = threads_per_row(p.dim);
+    if (tpr == 0) {
+        const int blocks = static_cast<int>(std::min<long long>(p.rows, 592));
+        if (!bwd) {
+            ln_fwd_long_kernel<T><<<blocks, kLong, 0, st>>>(p);
+        } else {
+            if (p.want_dx) ln_bwd_long_kernel<T><<<blocks, kLong, 0, st>>>(p);
+            if (p.want_part)
+                ln_cols_kernel<T><<<dim3((p.dim + 255) / 256, bwd_blocks(p.rows, p.dim)), 256, 0, st>>>(p);
+        }
+        return cudaGetLastError();
+    }
+    const long long rpb = tpr == 32 ? 4 : 1;
+    const int cap = tpr == 512 ? 296 : 1184;
+    const int blocks = bwd ? bwd_blocks(p.rows, p.dim)
+                           : static_cast<int>(std::min<long long>(cap, (p.rows + rpb - 1) / rpb));
+    // 16-byte pieces when every row starts on one and ends with one; else single elements, lane by lane.
+    const bool vec = p.dim % V == 0 && vec_ok<T, V>(p.x, p.xs, 0) &&
+                     (bwd ? vec_ok<T, V>(p.dy, p.dys, 0) && vec_ok<T, V>(p.dx, 0, 0) : vec_ok<T, V>(p.y, 0, 0));
+    const int per = (p.dim + tpr - 1) / tpr;  // features per thread
+    if (vec) {
+        const int nv = (per + V - 1) / V;
+        if constexpr (V == 8) {
+            if (nv <= 1) run_ln_t<T, V, 1>(p, tpr, bwd, blocks, st);
+            else if (nv == 2) run_ln_t<T, V, 2>(p, tpr, bwd, blocks, st);
+            else if (nv == 3) run_ln_t<T, V, 3>(p, tpr, bwd, blocks, st);
+            else run_ln_t<T, V, 4>(p, tpr, bwd, blocks, st);
+        } else {
+            if (nv <= 2) run_ln_t<T, V, 2>(p, tpr, bwd, blocks, st);
+            else if (nv <= 4) run_ln_t<T, V, 4>(p, tpr, bwd, blocks, st);
+            else if (nv <= 6) run_ln_t<T, V, 6>(p, tpr, bwd, blocks, st);
+            else run_ln_t<T, V, 8>(p, tpr, bwd, blocks, st);
+        }
+    } else {
+        if (per <= 8) run_ln_t<T, 1, 8>(p, tpr, bwd, blocks, st);
+        else if (per <= 16) run_ln_t<T, 1, 16>(p, tpr, bwd, blocks, st);
+        else run_ln_t<T, 1, 32>(p, tpr, bwd, blocks, st);
+    }
+    return cudaGetLastError();
+}
+
+LnP ln_params(const sdtw_layer_norm_args& a) {
+    LnP p{};
+    p.x = a.x;
+    p.dy = a.dy;
+    p.y = a.y;
+    p.dx = a.dx;
+    p.w = a.weight;
+    p.b = a.bias;
+    p.mean = a.mean;
+    p.rstd = a.rstd;
+    p.part = static_cast<float*>(a.workspace);
+    p.rows = a.rows;
+    p.xs = a.x_stride;
+    p.dys = a.dy_stride;
+    p.dim = a.dim;
+    p.eps = a.eps;
+    p.want_dx = a.dx != nullptr;
+    p.want_part = a.dweight || a.dbias;
+    return p;
+}
+
+cudaError_t run_ln_type(const sdtw_layer_norm_args& a, bool bwd, cudaStream_t st) {
+    const LnP p = ln_params(a);
+    if (a.dtype == SDTW_F32) return run_ln_all<float>(p, bwd, st);
+    if (a.dtype == SDTW_F16) return run_ln_all<__half>(p, bwd, st);
+    return run_ln_all<__nv_bfloat16>(p, bwd, st);
+}
+
+}  // namespace
+
+size_t layer_norm_bwd_ws(long long rows, int dim) {
+    return static_cast<size_t>(bwd_blocks(rows, dim)) * 2 * static_cast<size_t>(dim) * sizeof(float);
+}
+
+cudaError_t launch_layer_norm_fwd(const sdtw_layer_norm_args& a, cudaStream_t st) { return run_ln_type(a, false, st); }
+
+cudaError_t launch_layer_norm_bwd(const sdtw_layer_norm_args& a, cudaStream_t st) {
+    cudaError_t e = run_ln_type(a, true, st);
+    if (e != cudaSuccess || !(a.dweight || a.dbias)) return e;
+    return launch_pdl(true, ln_reduce_kernel, dim3((2 * a.dim + 31) / 32), dim3(32, 32), 0, st,
+                      static_cast<const float*>(a.workspace), bwd_blocks(a.rows, a.dim), a.dim, a.dweight, a.dbias);
+}
+
+}  // namespace sdtw

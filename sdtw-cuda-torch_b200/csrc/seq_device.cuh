@@ -1,0 +1,256 @@
+// seq_device.cuh -- device helpers of the sequence operators: element types,
+// vector loads and stores with a guarded fallback, lane reductions, packed
+// float32 pairs.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "sdtw_device.cuh"
+
+namespace sdtw {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// The 16-bit halves of a word as floats, and back.
+template <typename T>
+__device__ __forceinline__ float half_bits(uint32_t h);
+template <>
+__device__ __forceinline__ float half_bits<__half>(uint32_t h) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+}
+template <>
+__device__ __forceinline__ float half_bits<__nv_bfloat16>(uint32_t h) { return __uint_as_float(h << 16); }
+__device__ __forceinline__ uint32_t bits_of(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+
+// V elements in 32-bit words, moved in pieces of at most 16 bytes.  16-bit
+// elements are loaded as unsigned short: the headers' __ldg of __half and
+// __nv_bfloat16 is an asm statement without `volatile`, which the compiler may
+// move in front of the condition that guards it (seen as an illegal address
+// when the guarded pointer was null).
+template <typename T, int V>
+struct Vec {
+    static constexpr bool k32 = sizeof(T) == 4;
+    static constexpr int kWords = k32 ? V : (V + 1) / 2;
+    static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+    static constexpr int kPiece = kBytes < 16 ? kBytes : 16;  // bytes of one access
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (k32)
+            return __uint_as_float(w[e]);
+        else
+            return half_bits<T>(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+    }
+    // Elements must be set in order: an even one clears its word.
+    __device__ __forceinline__ void set(int e, float v) {
+        if constexpr (k32)
+            w[e] = __float_as_uint(v);
+        else if (e & 1)
+            w[e / 2] |= bits_of(from_f<T>(v)) << 16;
+        else
+            w[e / 2] = bits_of(from_f<T>(v));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kPiece == 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = q.x;
+                w[4 * i + 1] = q.y;
+                w[4 * i + 2] = q.z;
+                w[4 * i + 3] = q.w;
+            }
+        } else if constexpr (kPiece == 8) {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = q.x;
+            w[1] = q.y;
+        } else if constexpr (kPiece == 4) {
+            w[0] = __ldg(reinterpret_cast<const unsigned int*>(p));
+        } else {
+            w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kPiece == 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else if constexpr (kPiece == 8) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else if constexpr (kPiece == 4) {
+            *reinterpret_cast<unsigned int*>(p) = w[0];
+        } else {
+            *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(w[0]);
+        }
+    }
+    // n of the V elements exist at p (the others read as 0); `vec`: p is
+    // aligned for whole pieces and n is 0 or V.
+    __device__ __forceinline__ void load_n(const T* p, int n, bool vec) {
+        zero();
+        if (vec) {
+            if (n > 0) load(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) {
+                    if constexpr (k32)
+                        w[i] = __float_as_uint(__ldg(reinterpret_cast<const float*>(p) + i));
+                    else
+                        w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p) + i)) << (i & 1 ? 16 : 0);
+                }
+        }
+    }
+    __device__ __forceinline__ void store_n(T* p, int n, bool vec) const {
+        if (vec) {
+            if (n > 0) store(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) {
+                    if constexpr (k32)
+                        reinterpret_cast<float*>(p)[i] = __uint_as_float(w[i]);
+                    else
+                        reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
+                }
+        }
+    }
+};
+
+// Whether groups of V elements at p + (multiples of the strides and of V) can
+// be moved in Vec's pieces.
+template <typename T, int V>
+inline bool vec_ok(const void* p, long long s0, long long s1, long long s2 = 0) {
+    const uintptr_t piece = Vec<T, V>::kPiece;
+    return reinterpret_cast<uintptr_t>(p) % piece == 0 && (s0 * static_cast<long long>(sizeof(T))) % static_cast<long long>(piece) == 0 &&
+           (s1 * static_cast<long long>(sizeof(T))) % static_cast<long long>(piece) == 0 &&
+           (s2 * static_cast<long long>(sizeof(T))) % static_cast<long long>(piece) == 0;
+}
+
+// Logistic function: 1 / (1 + exp(-v)).  exp(-v) overflows to infinity below
+// v = -88.7, where the quotient is 0 as it should be.
+__device__ __forceinline__ float sigmoidf(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// log(1 + exp(v)) without overflow, and without losing exp(v) next to 1.
+__device__ __forceinline__ float softplusf(float v) { return fmaxf(v, 0.f) + log1pf(__expf(-fabsf(v))); }
+
+// Packed float32 pairs: halves the instructions of multiplies and adds.
+struct f2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ f2 pk(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void upk(f2 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ f2 ex22(f2 a) {
+    float x, y;
+    upk(a, x, y);
+    return pk(ex2f(x), ex2f(y));
+}
+__device__ __forceinline__ float sum2(f2 a) {
+    float x, y;
+    upk(a, x, y);
+    return x + y;
+}
+
+// Sums K values over the lanes that differ in bits LO .. LO * LANES / 2 of the
+// lane number.  While several values are left, each exchange halves them: a
+// lane keeps one half and sends the other.  Afterwards v[0 .. kept) are this
+// lane's sums of the values lane_slot(lane) + i.
+template <int K, int LO, int LANES>
+struct LaneSum {
+    static constexpr int kept = K > LANES ? K / LANES : 1;
+    __device__ static __forceinline__ void run(float (&v)[K], int lane) {
+        int n = K;
+#pragma unroll
+        for (int m = LO; m < LO * LANES; m *= 2) {
+            if (n > 1) {
+                n /= 2;
+                const bool up = lane & m;
+#pragma unroll
+                for (int i = 0; i < K / 2; ++i)
+                    if (i < n) {
+                        const float keep = up ? v[i + n] : v[i];
+                        const float send = up ? v[i] : v[i + n];
+                        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+                    }
+            } else {
+                v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+            }
+        }
+    }
+    // First value that this lane ends up with; lanes that differ only in bits
+    // beyond the halvings hold the same.
+    __device__ static __forceinline__ int slot(int lane) {
+        int n = K, s = 0;
+#pragma unroll
+        for (int m = LO; m < LO * LANES; m *= 2)
+            if (n > 1) {
+                n /= 2;
+                if (lane & m) s += n;
+            }
+        return s;
+    }
+    // One of the lanes that hold the same sums.
+    __device__ static __forceinline__ bool owner(int lane) {
+        int n = K;
+        bool own = true;
+#pragma unroll
+        for (int m = LO; m < LO * LANES; m *= 2) {
+            if (n > 1)
+                n /= 2;
+            else if (lane & m)
+                own = false;
+        }
+        return own;
+    }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
+}
+
+// Sequence length of batch entry b, clamped to [0, n].
+__device__ __forceinline__ int seq_len(const long long* lengths, int b, int n) {
+    if (lengths == nullptr) return n;
+    const long long l = lengths[b];
+    return l < 0 ? 0 : (l > n ? n : static_cast<int>(l));
+}
+
+}  // namespace sdtw

@@ -18,8 +18,10 @@ CSRC = os.path.join(ROOT, "csrc")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsdtw_b200.so")
 
-SOURCES = ["capi.cu", "wavefront.cu", "wavefront_exp.cu", "layout.cu", "dense.cu", "tcgemm.cu", "grad_small.cu", "barycenter.cu", "f64.cu", "cpu.cpp"]
-HEADERS = ["sdtw_device.cuh", "sdtw_kernels.h", "sdtw_plan.h", "wavefront_ring.cuh"]
+SOURCES = ["capi.cu", "wavefront.cu", "wavefront_exp.cu", "layout.cu", "dense.cu", "tcgemm.cu", "grad_small.cu", "barycenter.cu", "f64.cu", "cpu.cpp",
+           "layer_norm.cu", "causal_conv.cu", "selective_scan_fwd.cu", "selective_scan_bwd.cu"]
+HEADERS = ["sdtw_device.cuh", "sdtw_kernels.h", "sdtw_plan.h", "wavefront_ring.cuh", "seq_kernels.h", "seq_device.cuh",
+           "selective_scan.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -46,7 +48,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
     cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-fopenmp",
-           "-shared", "-o", tmp] + [os.path.join(CSRC, f) for f in SOURCES] + ["-lgomp"]
+           "--threads", "0", "-shared", "-o", tmp] + [os.path.join(CSRC, f) for f in SOURCES] + ["-lgomp"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), flush=True)

@@ -12,12 +12,16 @@ Functions.  Both routes make the same library calls.
   sq_forward / sq_backward   unfused path with the cost kept in the library's
                              layout (module.py:116-118 through autograd.py)
   d_forward / d_backward     arbitrary cost matrix D (autograd.py:11-48)
+  layer_norm_*, causal_conv_*, selective_scan_*
+                             the sequence operators (sequence.py)
 
 Float32, float16 and bfloat16 CUDA tensors (computed in float32, results in the
 input dtype).  The score (and cost) tables are flat float32 tensors in the
 library's layout, sized by ``_native.score_elems`` / ``cost_elems``.
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 from torch import Tensor
@@ -153,3 +157,176 @@ def _d_backward(ctx, grad_out, _grad_score):
 
 
 d_forward.register_autograd(_d_backward, setup_context=_d_setup)
+
+
+# ----------------------------------------------------------------------------- sequence operators
+def _need(ctx, n: int) -> list[bool]:
+    return [bool(v) for v in ctx.needs_input_grad[:n]]
+
+
+def _pack(grads, like: Tensor) -> list[Tensor]:
+    # A custom operator returns tensors only: an empty one stands for "not needed".
+    return [like.new_empty(_EMPTY) if g is None else g for g in grads]
+
+
+def _unpack(grads, inputs, need):
+    return [g.to(t.dtype) if n else None for g, t, n in zip(grads, inputs, need)]
+
+
+def _fake_grads(shapes, need, like: Tensor) -> list[Tensor]:
+    return [like.new_empty(s if n else _EMPTY, dtype=dt if n else like.dtype) for (s, dt), n in zip(shapes, need)]
+
+
+@torch.library.custom_op("softdtw_cuda::layer_norm_forward", mutates_args=(), device_types="cuda")
+def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
+                       eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    return _native.layer_norm_forward(x, weight, bias, eps)
+
+
+@layer_norm_forward.register_fake
+def _(x, weight, bias, eps):
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32))
+
+
+@torch.library.custom_op("softdtw_cuda::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward(x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, dy: Tensor,
+                        need: list[bool]) -> list[Tensor]:
+    return _pack(_native.layer_norm_backward(x, weight, mean, rstd, dy, *need), x)
+
+
+@layer_norm_backward.register_fake
+def _(x, weight, mean, rstd, dy, need):
+    D = (x.shape[-1],)
+    return _fake_grads(((x.shape, x.dtype), (D, torch.float32), (D, torch.float32)), need, x)
+
+
+def _ln_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+
+
+def _ln_backward(ctx, dy, _dmean, _drstd):
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    need = _need(ctx, 3)
+    return (*_unpack(layer_norm_backward(x, weight, mean, rstd, dy, need), (x, weight, bias), need), None)
+
+
+layer_norm_forward.register_autograd(_ln_backward, setup_context=_ln_setup)
+
+
+@torch.library.custom_op("softdtw_cuda::causal_conv_forward", mutates_args=(), device_types="cuda")
+def causal_conv_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, lengths: Optional[Tensor],
+                        initial_state: Optional[Tensor], want_state: bool) -> tuple[Tensor, Tensor]:
+    y, state = _native.conv_forward(x, weight, bias, silu, lengths, initial_state, want_state)
+    return y, (state if want_state else x.new_empty(_EMPTY))
+
+
+@causal_conv_forward.register_fake
+def _(x, weight, bias, silu, lengths, initial_state, want_state):
+    return x.new_empty(x.shape), x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2]) if want_state else _EMPTY)
+
+
+@torch.library.custom_op("softdtw_cuda::causal_conv_backward", mutates_args=(), device_types="cuda")
+def causal_conv_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, lengths: Optional[Tensor],
+                         initial_state: Optional[Tensor], dy: Tensor, dstate: Optional[Tensor],
+                         need: list[bool]) -> list[Tensor]:
+    return _pack(_native.conv_backward(x, weight, bias, silu, lengths, initial_state, dy, dstate, *need), x)
+
+
+@causal_conv_backward.register_fake
+def _(x, weight, bias, silu, lengths, initial_state, dy, dstate, need):
+    D, W, f32 = x.shape[2], weight.shape[1], torch.float32
+    return _fake_grads(((x.shape, x.dtype), ((D, W), f32), ((D,), f32), ((x.shape[0], W - 1, D), x.dtype)), need, x)
+
+
+def _conv_setup(ctx, inputs, output):
+    x, weight, bias, silu, lengths, initial_state, want_state = inputs
+    ctx.save_for_backward(x, weight, bias, lengths, initial_state)
+    ctx.silu, ctx.want_state = silu, want_state
+
+
+def _conv_backward(ctx, dy, dstate):
+    x, weight, bias, lengths, initial_state = ctx.saved_tensors
+    n = ctx.needs_input_grad
+    need = [bool(n[0]), bool(n[1]), bool(n[2]), bool(n[5])]
+    g = causal_conv_backward(x, weight, bias, ctx.silu, lengths, initial_state, dy, dstate if ctx.want_state else None, need)
+    gx, gw, gb, gs = _unpack(g, (x, weight, bias, initial_state), need)
+    return gx, gw, gb, None, None, gs, None
+
+
+causal_conv_forward.register_autograd(_conv_backward, setup_context=_conv_setup)
+
+
+@torch.library.custom_op("softdtw_cuda::causal_conv_step", mutates_args=("state", "state_out"), device_types="cuda")
+def causal_conv_step(x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, state: Tensor,
+                     state_out: Optional[Tensor]) -> Tensor:
+    return _native.conv_step(x, weight, bias, silu, state, state if state_out is None else state_out)
+
+
+@causal_conv_step.register_fake
+def _(x, weight, bias, silu, state, state_out):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("softdtw_cuda::selective_scan_forward", mutates_args=(), device_types="cuda")
+def selective_scan_forward(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                           z: Optional[Tensor], delta_bias: Optional[Tensor], softplus: bool, lengths: Optional[Tensor],
+                           initial_state: Optional[Tensor], want_state: bool, save: bool) -> tuple[Tensor, Tensor, Tensor]:
+    y, state, saved = _native.scan_forward(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state,
+                                           want_state, save)
+    empty = A.new_empty(_EMPTY, dtype=torch.float32)
+    return y, (state if want_state else empty), (saved if save else torch.empty_like(empty))
+
+
+@selective_scan_forward.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state, want_state, save):
+    Bt, N, Dm = x.shape
+    S, f32 = A.shape[1], torch.float32
+    return (x.new_empty(x.shape), x.new_empty((Bt, Dm, S) if want_state else _EMPTY, dtype=f32),
+            x.new_empty((_native.scan_saved_elems(Bt, N, Dm, S),) if save else _EMPTY, dtype=f32))
+
+
+@torch.library.custom_op("softdtw_cuda::selective_scan_backward", mutates_args=(), device_types="cuda")
+def selective_scan_backward(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                            z: Optional[Tensor], delta_bias: Optional[Tensor], softplus: bool, lengths: Optional[Tensor],
+                            saved: Tensor, dy: Tensor, dstate: Optional[Tensor], need: list[bool]) -> list[Tensor]:
+    return _pack(_native.scan_backward(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, saved, dy, dstate, need), x)
+
+
+@selective_scan_backward.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, saved, dy, dstate, need):
+    Dm, S, f32 = x.shape[2], A.shape[1], torch.float32
+    return _fake_grads(((x.shape, x.dtype), (x.shape, x.dtype), ((Dm, S), f32), (B.shape, x.dtype), (B.shape, x.dtype),
+                        ((Dm,), f32), (x.shape, x.dtype), ((Dm,), f32), ((x.shape[0], Dm, S), f32)), need, x)
+
+
+def _scan_setup(ctx, inputs, output):
+    x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state, want_state, _ = inputs
+    ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, initial_state, output[2])
+    ctx.softplus, ctx.want_state = softplus, want_state
+
+
+def _scan_backward(ctx, dy, dstate, _dsaved):
+    x, delta, A, B, C, D, z, delta_bias, lengths, initial_state, saved = ctx.saved_tensors
+    n = ctx.needs_input_grad
+    need = [bool(v) for v in (*n[:8], n[10])]
+    g = selective_scan_backward(x, delta, A, B, C, D, z, delta_bias, ctx.softplus, lengths, saved, dy,
+                                dstate if ctx.want_state else None, need)
+    g = _unpack(g, (x, delta, A, B, C, D, z, delta_bias, initial_state), need)
+    return (*g[:8], None, None, g[8], None, None)
+
+
+selective_scan_forward.register_autograd(_scan_backward, setup_context=_scan_setup)
+
+
+@torch.library.custom_op("softdtw_cuda::selective_scan_step", mutates_args=("state", "state_out"), device_types="cuda")
+def selective_scan_step(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                        z: Optional[Tensor], delta_bias: Optional[Tensor], softplus: bool, state: Tensor,
+                        state_out: Optional[Tensor]) -> Tensor:
+    return _native.scan_step(x, delta, A, B, C, D, z, delta_bias, softplus, state, state if state_out is None else state_out)
+
+
+@selective_scan_step.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, softplus, state, state_out):
+    return x.new_empty(x.shape)

@@ -1,0 +1,471 @@
+"""Sequence operators with gradients: the layers of a model of series.
+
+``SoftDTW`` compares series (B, N, D); these operators make them.  All take
+series with time second to last and features last, and parameters as torch's
+own layers keep them:
+
+  layer_norm            normalisation over the features of each time step
+  causal_conv           short causal convolution of each feature over time
+  selective_scan        selective state space recurrence over time
+  causal_conv_step,     one new time step of running series, from the states
+  selective_scan_step   that the two return
+
+CUDA tensors of float32, float16 or bfloat16 run the library's kernels
+(float32 arithmetic and states, results in the input type); float64 and CPU
+tensors, and empty ones, use the same formulas in plain torch ops.  No
+counterpart in the reference package.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from .distances import _KERNEL_DTYPES
+from .utils.checks import _FLOAT_DTYPES
+
+MAX_WIDTH = 8
+MAX_STATE = 64
+
+
+# ----------------------------------------------------------------------------- checks
+def _check_series(name: str, t: Tensor, like: Tensor | None = None, shape: tuple | None = None) -> None:
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must have x's dtype {like.dtype}, got {t.dtype}")
+        if t.device != like.device:
+            raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
+
+
+def _check_param(name: str, t: Tensor | None, like: Tensor, shape: tuple) -> None:
+    if t is None:
+        return
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
+
+
+def _check_lengths(lengths, x: Tensor) -> Tensor | None:
+    if lengths is None:
+        return None
+    if not isinstance(lengths, Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError("lengths must be an int32 or int64 tensor")
+    if lengths.device != x.device:
+        raise ValueError(f"lengths must be on x's device {x.device}, got {lengths.device}")
+    if tuple(lengths.shape) != (x.shape[0],):
+        raise ValueError(f"lengths must have shape ({x.shape[0]},). Got {tuple(lengths.shape)}")
+    return lengths.to(torch.int64).contiguous()
+
+
+def _check_state(name: str, t: Tensor, like: Tensor, shape: tuple, dtype: torch.dtype) -> None:
+    """A running state: each batch entry contiguous, entries apart from each other."""
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
+    if t.numel() and (not t[0].is_contiguous() or (shape[0] > 1 and t.stride(0) < t[0].numel())):
+        raise ValueError(f"{name} must hold each batch entry contiguously, got strides {t.stride()}")
+
+
+def _check_state_pair(state: Tensor, out: Tensor) -> None:
+    """The new state may be written over the old one, but not over a part of it."""
+    if out is state or not state.numel():
+        return
+    B, inner, size = state.shape[0], state[0].numel(), state.element_size()
+    s0, o0 = state.data_ptr(), out.data_ptr()
+    ss, so = state.stride(0), out.stride(0)
+    if s0 == o0 and (ss == so or B == 1):
+        return
+    s1, o1 = s0 + ((B - 1) * ss + inner) * size, o0 + ((B - 1) * so + inner) * size
+    if s1 <= o0 or o1 <= s0:
+        return
+    if ss == so and B > 1 and inner * size <= (o0 - s0) % (ss * size) <= (ss - inner) * size:
+        return  # interleaved entries of one larger tensor
+    raise ValueError("state_out overlaps state")
+
+
+def _check_inference(what: str, *tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
+
+
+def _silu_flag(activation) -> bool:
+    if activation not in (None, "silu"):
+        raise ValueError(f"Unknown activation={activation!r}. Supported: None, 'silu'")
+    return activation == "silu"
+
+
+def _on_kernels(x: Tensor) -> bool:
+    return x.is_cuda and x.dtype in _KERNEL_DTYPES and x.numel() > 0
+
+
+def _tracked(*tensors: Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _wide(t: Tensor | None) -> Tensor | None:
+    # float32 for 16-bit tensors, as the kernels compute.
+    return None if t is None else (t if t.dtype == torch.float64 else t.float())
+
+
+def _grad_as(g: Tensor | None, like: Tensor | None) -> Tensor | None:
+    return None if g is None else g.to(like.dtype)
+
+
+# ----------------------------------------------------------------------------- layer norm
+class _LayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _native.layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        dx, dw, db = _native.layer_norm_backward(x, weight, mean, rstd, dy, *ctx.needs_input_grad[:3])
+        return dx, _grad_as(dw, weight), _grad_as(db, bias), None
+
+
+def _layer_norm_torch(x, weight, bias, eps):
+    v = _wide(x)
+    c = v - v.mean(-1, keepdim=True)
+    v = c * torch.rsqrt((c * c).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        v = v * weight.to(v.dtype)
+    if bias is not None:
+        v = v + bias.to(v.dtype)
+    return v.to(x.dtype)
+
+
+def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, *, eps: float = 1e-5) -> Tensor:
+    """Layer norm over the last dimension of x (..., D): (x - mean) / sqrt(var + eps) * weight + bias.
+
+    weight, bias  (D,), or None for 1 and 0; gradients flow to all three
+    """
+    _check_series("x", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have a last dimension > 0. Got {tuple(x.shape)}")
+    D = x.shape[-1]
+    _check_param("weight", weight, x, (D,))
+    _check_param("bias", bias, x, (D,))
+    eps = float(eps)
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    if not _on_kernels(x):
+        return _layer_norm_torch(x, weight, bias, eps)
+    if torch.compiler.is_compiling():
+        return torch.ops.softdtw_cuda.layer_norm_forward(x, weight, bias, eps)[0]
+    if _tracked(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _native.layer_norm_forward(x, weight, bias, eps, stats=False)[0]
+
+
+# ----------------------------------------------------------------------------- causal convolution
+class _CausalConv(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial_state, lengths, silu, want_state):
+        y, state = _native.conv_forward(x, weight, bias, silu, lengths, initial_state, want_state)
+        ctx.save_for_backward(x, weight, bias, initial_state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, state
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate):
+        x, weight, bias, initial_state, lengths = ctx.saved_tensors
+        if dy is None:
+            if dstate is None:
+                return (None,) * 7
+            dy = torch.zeros_like(x)
+        nx, nw, nb, ns = ctx.needs_input_grad[:4]
+        dx, dw, db, ds = _native.conv_backward(x, weight, bias, ctx.silu, lengths, initial_state, dy, dstate, nx, nw,
+                                               nb, ns)
+        return dx, _grad_as(dw, weight), _grad_as(db, bias), ds, None, None, None
+
+
+def _causal_conv_torch(x, weight, bias, silu, lengths, initial_state):
+    B, N, D = x.shape
+    W = weight.shape[1]
+    v = _wide(x)
+    live = None
+    if lengths is not None:
+        lengths = lengths.clamp(0, N)
+        live = (torch.arange(N, device=x.device)[None, :] < lengths[:, None])[..., None]
+        v = torch.where(live, v, v.new_zeros(()))
+    past = v.new_zeros(B, W - 1, D) if initial_state is None else initial_state.to(v.dtype)
+    s = torch.cat([past, v], dim=1)
+    w = weight.to(v.dtype)
+    y = s[:, :N] * w[:, 0]
+    for k in range(1, W):
+        y = y + s[:, k:k + N] * w[:, k]
+    if bias is not None:
+        y = y + bias.to(v.dtype)
+    if silu:
+        y = y * torch.sigmoid(y)
+    if live is not None:
+        y = torch.where(live, y, y.new_zeros(()))
+    first = torch.full((B,), N, device=x.device) if lengths is None else lengths
+    at = (first[:, None] + torch.arange(W - 1, device=x.device)[None, :])[..., None].expand(B, W - 1, D)
+    return y.to(x.dtype), torch.gather(s, 1, at).to(x.dtype)
+
+
+def _check_conv_weight(x, weight, bias):
+    D = x.shape[-1]
+    if not isinstance(weight, Tensor) or weight.dim() != 2 or weight.shape[0] != D:
+        raise ValueError(f"weight must have shape ({D}, W). Got {tuple(getattr(weight, 'shape', ()))}")
+    W = weight.shape[1]
+    if not 1 <= W <= MAX_WIDTH:
+        raise ValueError(f"weight's width must be between 1 and {MAX_WIDTH}, got {W}")
+    _check_param("weight", weight, x, (D, W))
+    _check_param("bias", bias, x, (D,))
+    return W
+
+
+def causal_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation: str | None = None,
+                lengths: Tensor | None = None, initial_state: Tensor | None = None, return_state: bool = False):
+    """Causal convolution of each feature of x (B, N, D) with its own weights (D, W), W <= 8:
+
+        y[:, t] = activation(bias + sum_k weight[:, k] * x[:, t - W + 1 + k])
+
+    activation     None or "silu"
+    lengths        (B,) valid steps of each series (clamped to [0, N]); steps beyond are not read, their
+                   outputs and gradients are 0
+    initial_state  (B, W - 1, D) inputs before the series, of x's dtype; None = zeros
+    return_state   also return the last W - 1 inputs of each series (B, W - 1, D), for
+                   ``causal_conv_step`` or as the next ``initial_state``
+    """
+    _check_series("x", x)
+    if x.dim() != 3 or x.shape[2] == 0:
+        raise ValueError(f"x must have shape (B, N, D) with D > 0. Got {tuple(x.shape)}")
+    W = _check_conv_weight(x, weight, bias)
+    silu = _silu_flag(activation)
+    lengths = _check_lengths(lengths, x)
+    if initial_state is not None:
+        _check_series("initial_state", initial_state, x, (x.shape[0], W - 1, x.shape[2]))
+    if not _on_kernels(x):
+        y, state = _causal_conv_torch(x, weight, bias, silu, lengths, initial_state)
+    elif torch.compiler.is_compiling():
+        y, state = torch.ops.softdtw_cuda.causal_conv_forward(x, weight, bias, silu, lengths, initial_state, return_state)
+    elif _tracked(x, weight, bias, initial_state):
+        y, state = _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, return_state)
+    else:
+        y, state = _native.conv_forward(x, weight, bias, silu, lengths, initial_state, return_state)
+    return (y, state) if return_state else y
+
+
+def causal_conv_step(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, state: Tensor,
+                     activation: str | None = None, state_out: Tensor | None = None) -> Tensor:
+    """One new time step x (B, D) of running series: y (B, D) as ``causal_conv`` gives it.
+
+    state      (B, W - 1, D) of x's dtype, the inputs before x; moved up by x in place
+    state_out  takes the new state instead, and ``state`` stays as it is
+
+    Not differentiable.
+    """
+    _check_series("x", x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must have shape (B, D) with D > 0. Got {tuple(x.shape)}")
+    W = _check_conv_weight(x, weight, bias)
+    silu = _silu_flag(activation)
+    shape = (x.shape[0], W - 1, x.shape[1])
+    _check_state("state", state, x, shape, x.dtype)
+    out = state if state_out is None else state_out
+    _check_state("state_out", out, x, shape, x.dtype)
+    _check_state_pair(state, out)
+    _check_inference("causal_conv_step", x, weight, bias, state, out)
+    if _on_kernels(x):
+        if torch.compiler.is_compiling():
+            return torch.ops.softdtw_cuda.causal_conv_step(x, weight, bias, silu, state, state_out)
+        y = _native.conv_step(x, weight, bias, silu, state, out)
+        torch.autograd.graph.increment_version(out)
+        return y
+    y, new = _causal_conv_torch(x[:, None], weight, bias, silu, None, state)
+    out.copy_(new)
+    return y[:, 0]
+
+
+# ----------------------------------------------------------------------------- selective scan
+class _SelectiveScan(Function):
+    @staticmethod
+    def forward(ctx, x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softplus, want_state):
+        y, state, saved = _native.scan_forward(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state,
+                                               want_state, True)
+        ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, saved)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, state
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate):
+        x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, saved = ctx.saved_tensors
+        if dy is None:
+            if dstate is None:
+                return (None,) * 12
+            dy = torch.zeros_like(x)
+        g = _native.scan_backward(x, delta, A, B, C, D, z, delta_bias, ctx.softplus, lengths, saved, dy, dstate,
+                                  ctx.needs_input_grad[:9])
+        for i, like in ((2, A), (5, D), (7, delta_bias), (8, initial_state)):
+            g[i] = _grad_as(g[i], like)
+        return (*g, None, None, None)
+
+
+def _selective_scan_torch(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state):
+    Bt, N, Dm = x.shape
+    G, S = B.shape[2], A.shape[1]
+    v, dt, B, C = _wide(x), _wide(delta), _wide(B), _wide(C)
+    A = A.to(v.dtype)
+    live, zero = None, v.new_zeros(())
+    if lengths is not None:
+        # Masked on both sides of each function: a NaN in the padding would come back through its derivative.
+        live = (torch.arange(N, device=x.device)[None, :] < lengths[:, None])[..., None]
+        v, dt = torch.where(live, v, zero), torch.where(live, dt, zero)
+        B, C = torch.where(live[..., None], B, zero), torch.where(live[..., None], C, zero)
+    if delta_bias is not None:
+        dt = dt + delta_bias.to(v.dtype)
+    if softplus:
+        dt = torch.logaddexp(dt, zero)
+    if live is not None:
+        dt = torch.where(live, dt, zero)
+    h = v.new_zeros(Bt, Dm, S) if initial_state is None else initial_state.to(v.dtype)
+    u = dt * v
+    ys = []
+    for t in range(N):
+        Bx, Cx = (m[:, t, :, None].expand(Bt, G, Dm // G, S).reshape(Bt, Dm, S) for m in (B, C))
+        h = torch.exp(dt[:, t, :, None] * A) * h + u[:, t, :, None] * Bx
+        ys.append((h * Cx).sum(-1))
+    y = torch.stack(ys, 1) if ys else v.new_zeros(Bt, 0, Dm)
+    if D is not None:
+        y = y + v * D.to(v.dtype)
+    if z is not None:
+        zw = _wide(z)
+        if live is not None:
+            zw = torch.where(live, zw, zero)
+        y = y * zw * torch.sigmoid(zw)
+    if live is not None:
+        y = torch.where(live, y, zero)
+    return y.to(x.dtype), h
+
+
+def _check_scan(x, delta, A, B, C, D, z, delta_bias, seq: tuple):
+    Dm = x.shape[-1]
+    _check_series("delta", delta, x, tuple(x.shape))
+    if z is not None:
+        _check_series("z", z, x, tuple(x.shape))
+    if not isinstance(A, Tensor) or A.dim() != 2 or A.shape[0] != Dm:
+        raise ValueError(f"A must have shape ({Dm}, S). Got {tuple(getattr(A, 'shape', ()))}")
+    S = A.shape[1]
+    if not 1 <= S <= MAX_STATE:
+        raise ValueError(f"A's state size must be between 1 and {MAX_STATE}, got {S}")
+    _check_param("A", A, x, (Dm, S))
+    _check_series("B", B, x)
+    _check_series("C", C, x)
+    n = len(seq)
+    if B.dim() not in (n + 1, n + 2) or tuple(B.shape[:n]) != seq or B.shape[-1] != S:
+        raise ValueError(f"B must have shape {(*seq, S)} or {(*seq, 'G', S)}. Got {tuple(B.shape)}")
+    if B.dim() == n + 2 and (B.shape[n] == 0 or Dm % B.shape[n]):
+        raise ValueError(f"B's groups ({B.shape[n]}) must divide the features ({Dm})")
+    _check_series("C", C, x, tuple(B.shape))
+    _check_param("D", D, x, (Dm,))
+    _check_param("delta_bias", delta_bias, x, (Dm,))
+    if B.dim() == n + 1:
+        B, C = B.unsqueeze(n), C.unsqueeze(n)
+    return B, C, S
+
+
+def selective_scan(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, *, D: Tensor | None = None,
+                   z: Tensor | None = None, delta_bias: Tensor | None = None, delta_softplus: bool = False,
+                   lengths: Tensor | None = None, initial_state: Tensor | None = None, return_state: bool = False):
+    """Selective state space recurrence over the time steps of x (Bt, N, Dm), with S <= 64 states per feature:
+
+        dt = delta + delta_bias, or softplus of it with ``delta_softplus``
+        h  = exp(dt * A) * h + dt * B[:, t] * x[:, t]              (Bt, Dm, S)
+        y[:, t] = sum over S of C[:, t] * h  +  D * x[:, t],       times z * sigmoid(z) with ``z``
+
+    delta, z       (Bt, N, Dm)
+    A              (Dm, S), usually negative
+    B, C           (Bt, N, S), or (Bt, N, G, S) with a set for each of G groups of Dm / G features
+    D, delta_bias  (Dm,) or None
+    lengths        (Bt,) valid steps of each series (clamped to [0, N]); steps beyond are not read, their
+                   outputs and gradients are 0, and the state stays as the last valid step left it
+    initial_state  (Bt, Dm, S); None = zeros
+    return_state   also return the last state (Bt, Dm, S) in float32 (float64 for float64 inputs), for
+                   ``selective_scan_step`` or as the next ``initial_state``
+
+    x, delta, B, C and z share one dtype; A, D, delta_bias and the states are computed in float32.
+    """
+    _check_series("x", x)
+    if x.dim() != 3 or x.shape[2] == 0:
+        raise ValueError(f"x must have shape (B, N, D) with D > 0. Got {tuple(x.shape)}")
+    B, C, S = _check_scan(x, delta, A, B, C, D, z, delta_bias, (x.shape[0], x.shape[1]))
+    lengths = _check_lengths(lengths, x)
+    softplus = bool(delta_softplus)
+    _check_param("initial_state", initial_state, x, (x.shape[0], x.shape[2], S))
+    if not _on_kernels(x):
+        y, state = _selective_scan_torch(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state)
+    elif torch.compiler.is_compiling():
+        save = _tracked(x, delta, A, B, C, D, z, delta_bias, initial_state)
+        y, state, _ = torch.ops.softdtw_cuda.selective_scan_forward(x, delta, A, B, C, D, z, delta_bias, softplus, lengths,
+                                                                    initial_state, return_state, save)
+    elif _tracked(x, delta, A, B, C, D, z, delta_bias, initial_state):
+        y, state = _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softplus,
+                                        return_state)
+    else:
+        y, state, _ = _native.scan_forward(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state,
+                                           return_state, False)
+    return (y, state) if return_state else y
+
+
+def selective_scan_step(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, *, state: Tensor,
+                        D: Tensor | None = None, z: Tensor | None = None, delta_bias: Tensor | None = None,
+                        delta_softplus: bool = False, state_out: Tensor | None = None) -> Tensor:
+    """One new time step x, delta, z (Bt, Dm), B, C (Bt, S) or (Bt, G, S) of running series: y (Bt, Dm).
+
+    state      (Bt, Dm, S) float32 (float64 for float64 inputs), as ``selective_scan`` returns it; advanced in place
+    state_out  takes the new state instead, and ``state`` stays as it is
+
+    Not differentiable.
+    """
+    _check_series("x", x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must have shape (B, D) with D > 0. Got {tuple(x.shape)}")
+    B, C, S = _check_scan(x, delta, A, B, C, D, z, delta_bias, (x.shape[0],))
+    shape = (x.shape[0], x.shape[1], S)
+    st_dtype = torch.float64 if x.dtype == torch.float64 else torch.float32
+    _check_state("state", state, x, shape, st_dtype)
+    out = state if state_out is None else state_out
+    _check_state("state_out", out, x, shape, st_dtype)
+    _check_state_pair(state, out)
+    _check_inference("selective_scan_step", x, delta, A, B, C, D, z, delta_bias, state, out)
+    softplus = bool(delta_softplus)
+    if _on_kernels(x):
+        if torch.compiler.is_compiling():
+            return torch.ops.softdtw_cuda.selective_scan_step(x, delta, A, B, C, D, z, delta_bias, softplus, state,
+                                                              state_out)
+        y = _native.scan_step(x, delta, A, B, C, D, z, delta_bias, softplus, state, out)
+        torch.autograd.graph.increment_version(out)
+        return y
+    one = [None if t is None else t[:, None] for t in (x, delta, B, C, z)]
+    y, new = _selective_scan_torch(one[0], one[1], A, one[2], one[3], D, one[4], delta_bias, softplus, None, state)
+    out.copy_(new)
+    return y[:, 0]
