@@ -393,7 +393,7 @@ int sdtw_conv_step(const sdtw_conv_args *args, void *stream);
  * with the group g = d / (dim / groups).  h starts as state_in (NULL = zeros);
  * state_out, if given, gets h after each series' last valid step.  `saved`
  * (sdtw_scan_saved_elems floats; NULL when no backward follows) keeps the state
- * every 32 steps for the backward, which writes the gradients of every input
+ * every 8 or 16 steps for the backward, which writes the gradients of every input
  * (d* fields, each optional) from dy and dstate_out (optional).
  * sdtw_scan_step is the length-1 form for a running state:
  * state_in and state_out may be the same tensor, and lengths is not used. */
@@ -419,10 +419,11 @@ typedef struct {
     void *dB, *dC;             /* backward: (batch, length, groups, nstate) contiguous, optional */
     float *dA, *dD, *ddelta_bias; /* backward: contiguous, optional */
     float *dstate_in;          /* backward: contiguous, optional */
-    void *workspace;           /* backward: sdtw_scan_workspace_bytes */
+    void *workspace;           /* sdtw_scan_forward_workspace_bytes (may be 0), backward: sdtw_scan_workspace_bytes */
     size_t workspace_bytes;
 } sdtw_scan_args;
 size_t sdtw_scan_saved_elems(int batch, int length, int dim, int nstate);
+size_t sdtw_scan_forward_workspace_bytes(int batch, int length, int dim, int groups, int nstate);
 size_t sdtw_scan_workspace_bytes(int batch, int length, int dim, int groups, int nstate);
 int sdtw_scan_forward(const sdtw_scan_args *args, void *stream);
 int sdtw_scan_backward(const sdtw_scan_args *args, void *stream);

@@ -1445,16 +1445,23 @@ size_t sdtw_scan_saved_elems(int batch, int length, int dim, int nstate) {
     return batch <= 0 || length <= 0 || dim <= 0 || nstate <= 0 ? 0 : scan_states(batch, length, dim, nstate);
 }
 
+static bool scan_sizes_ok(int batch, int length, int dim, int groups, int nstate) {
+    return batch > 0 && length > 0 && dim > 0 && groups > 0 && nstate > 0 && nstate <= kScanMaxState && dim % groups == 0;
+}
+size_t sdtw_scan_forward_workspace_bytes(int batch, int length, int dim, int groups, int nstate) {
+    return scan_sizes_ok(batch, length, dim, groups, nstate) ? scan_fwd_ws(batch, length, dim, groups, nstate) : 0;
+}
 size_t sdtw_scan_workspace_bytes(int batch, int length, int dim, int groups, int nstate) {
-    if (batch <= 0 || length <= 0 || dim <= 0 || groups <= 0 || nstate <= 0 || nstate > kScanMaxState || dim % groups) return 0;
-    return scan_bwd_ws(batch, length, dim, groups, nstate);
+    return scan_sizes_ok(batch, length, dim, groups, nstate) ? scan_bwd_ws(batch, length, dim, groups, nstate) : 0;
 }
 
 int sdtw_scan_forward(const sdtw_scan_args* a, void* stream) {
     return guarded([&] {
         if (int rc = check_scan(a)) return rc;
         if (!a->y) return null_pointer();
-        return run_kernels("scan_fwd", 1, stream, [&](cudaStream_t st) { return launch_scan_fwd(*a, st); });
+        const size_t need = scan_fwd_ws(a->batch, a->length, a->dim, a->groups, a->nstate);
+        if (int rc = check_workspace(a->workspace, a->workspace_bytes, need)) return rc;
+        return run_kernels("scan_fwd", need ? 2 : 1, stream, [&](cudaStream_t st) { return launch_scan_fwd(*a, st); });
     });
 }
 
@@ -1465,7 +1472,8 @@ int sdtw_scan_backward(const sdtw_scan_args* a, void* stream) {
         if (int rc = check_workspace(a->workspace, a->workspace_bytes,
                                      scan_bwd_ws(a->batch, a->length, a->dim, a->groups, a->nstate)))
             return rc;
-        return run_kernels("scan_bwd", 2, stream, [&](cudaStream_t st) { return launch_scan_bwd(*a, st); });
+        const bool split = scan_split(a->batch, a->length, a->dim, a->groups, a->nstate, true).nseg > 1;
+        return run_kernels("scan_bwd", split ? 3 : 2, stream, [&](cudaStream_t st) { return launch_scan_bwd(*a, st); });
     });
 }
 

@@ -169,12 +169,6 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
     }
 }
 
-// Derivative of v sigmoid(v).
-__device__ __forceinline__ float dsilu(float v) {
-    const float sg = sigmoidf(v);
-    return sg * (1.f + v * (1.f - sg));
-}
-
 template <typename T, int VEC, int WT>
 __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
     constexpr int KM = Width<WT>::kMax;

@@ -1,5 +1,5 @@
 // selective_scan.cuh -- what the forward and the backward of the selective
-// scan share: the tiling, the staging of a warp's time steps, the kernel block.
+// scan share: the tiling, the split of the time axis, the kernel block.
 //
 //   dt = softplus(delta + bias),  u = dt x,  a[n] = exp(dt A[n])
 //   h[n] <- a[n] h[n] + u B[n],   y = sum_n C[n] h[n] + D x,   out = y z sigmoid(z)
@@ -8,15 +8,16 @@
 // lanes side by side cover up to 4 NL states and the 32 / NL lane groups 64 / NL
 // features.  So B and C (one row of states per time step, shared by the
 // features) cost one 16-byte shared-memory load each per 8 state updates, dt and
-// u another, and the sums over the states are log2(NL) lane exchanges.
+// u another, and the sums over the states are log2(NL) lane exchanges.  A warp
+// walks over the time steps; dt, u, B and C of TS steps at a time are staged in
+// shared memory, the elementwise functions computed once per element there.
 //
-// Time.  The warps of a block hold consecutive runs of 8 steps of the same
-// features.  Each computes its run's exponentials once and keeps them in
-// registers, runs the recurrence from h = 0, and publishes the run's product of
-// decays P and end state E: h_out = P h_in + E.  After one barrier every warp
-// chains the runs before its own and runs its steps again from the true state
-// with the decays that it kept.  The exponentials, which bound the kernel (16
-// per SM and cycle), are computed once each whatever the number of warps.
+// Time.  When there are too few warps to fill the GPU, the time axis is cut into
+// segments: a first kernel runs each from h = 0 and keeps its end state E and
+// the sum of its dt (whose exponential with A is the product of the decays), and
+// the main kernel's warps chain the segments before their own,
+// h <- exp(A sum dt) h + E, before they start.  The exponentials are then
+// computed twice.
 #pragma once
 
 #include "seq_device.cuh"
@@ -24,48 +25,62 @@
 
 namespace sdtw {
 
-constexpr int kScanSteps = 8;                        // time steps of a warp's run
-constexpr int kScanWarps = kScanChunk / kScanSteps;  // 4
+constexpr int kScanWarps = 4;
 constexpr int kScanThreads = 32 * kScanWarps;
-constexpr int kCT = 2;  // features per thread
+constexpr int kCT = 2;     // features per thread
+constexpr int kRun = 8;    // time steps held in registers
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int NL>
 struct ScanTile {
-    static constexpr int CL = 32 / NL;     // lane groups over features
-    static constexpr int CH = CL * kCT;    // features per block
-    static constexpr int NP = 4 * NL;      // states, padded
-    static constexpr int VX = CH / 4;      // features of a staging lane (4 lanes per time step)
-    static constexpr int VN = NL;          // states of a staging lane
+    static constexpr int CL = 32 / NL;               // lane groups over features
+    static constexpr int CH = CL * kCT;              // features per warp
+    static constexpr int NP = 4 * NL;                // states, padded
+    static constexpr int TS = scan_stage_steps(NL);  // staged time steps
+    static constexpr int LR = 32 / TS;               // staging lanes per time step
+    static constexpr int VX = CH / LR;               // features of a staging lane
+    static constexpr int VN = NP / LR;               // states of a staging lane
 };
 
 struct ScanP {
     sdtw_scan_args a;
-    int dg;       // features per group
-    int tiles_g;  // blocks per group
-    int nchunk;
+    int dg;        // features per group
+    int tiles_g;   // warps' tiles per group
+    int nchunk;    // stored states per series
+    int nseg, seglen;
     bool vec_x, vec_delta, vec_z, vec_B, vec_C, vec_y, vec_dy, vec_dx, vec_ddelta, vec_dz;
-    bool vec_n;   // the states of a thread are 16 bytes aligned
-    float* part_bc;   // (tiles, batch, length, 2, NP) partial dB, dC
-    float* part_par;  // (batch, dim * nstate + 2 * dim) partial dA, dD, ddelta_bias
+    bool vec_n;    // the states of a thread are 16 bytes aligned
+    float* seg_dt;    // (batch, nseg, dim) sums of dt
+    float* seg_E;     // (batch, nseg, dim, nstate) end states of the segments run from 0
+    float* part_bc;   // backward: (blocks over features, batch, length, 2, NP) partial dB, dC
+    float* part_par;  // backward: (batch, nseg, dim * nstate + 2 * dim) partial dA, dD, ddelta_bias
 };
 
-// The block's place: batch entry, first feature and how many of them exist.
+// A warp's place.  `tile` counts the warps over the features, all groups.
 template <int NL>
 struct ScanPlace {
-    int b, tile, g, c0, nc;
-    __device__ __forceinline__ explicit ScanPlace(const ScanP& p) {
-        const int tiles = p.tiles_g * p.a.groups;
-        b = blockIdx.x / tiles;
-        tile = blockIdx.x % tiles;
-        g = tile / p.tiles_g;
-        const int first = (tile % p.tiles_g) * ScanTile<NL>::CH;
+    int b, seg, g, c0, nc;
+    int t0, t1;  // the segment
+    __device__ __forceinline__ ScanPlace(const ScanP& p, int batch, int segment, int group, int tile_in_group) {
+        b = batch;
+        seg = segment;
+        g = group;
+        const int first = tile_in_group * ScanTile<NL>::CH;
         c0 = g * p.dg + first;
-        nc = min(ScanTile<NL>::CH, p.dg - first);
+        nc = max(0, min(ScanTile<NL>::CH, p.dg - first));
+        t0 = seg * p.seglen;
+        t1 = min(t0 + p.seglen, p.a.length);
+    }
+    __device__ static __forceinline__ ScanPlace of_warp(const ScanP& p, long long i) {
+        const int tiles = p.tiles_g * p.a.groups;
+        const int tile = static_cast<int>(i % tiles);
+        const long long bs = i / tiles;
+        return ScanPlace(p, static_cast<int>(bs / p.nseg), static_cast<int>(bs % p.nseg), tile / p.tiles_g, tile % p.tiles_g);
     }
 };
 
-// A thread's 4 states of 2 features, as pairs [feature][pair].
+// A thread's 4 states of 2 features, as pairs [feature][pair].  Lanes with an
+// odd state group hold their two features swapped (see pair_exchange).
 struct St {
     f2 v[kCT][2];
 };
@@ -73,51 +88,51 @@ __device__ __forceinline__ void st_set(St& s, float x) {
 #pragma unroll
     for (int i = 0; i < kCT; ++i) s.v[i][0] = s.v[i][1] = pk(x, x);
 }
-// s <- P s + E with the run's P and E in shared memory ([feature][lane]).
-__device__ __forceinline__ void st_chain(St& s, const ulonglong2 (*P)[32], const ulonglong2 (*E)[32], int lane) {
+// States n0 .. n0 + 4 of features f + (0 ^ swap) and f + (1 ^ swap) of a
+// (features, S) table; those that do not exist read as 0 and are not written.
+__device__ __forceinline__ void st_load(St& s, const float* tab, int f, int swap, int nf, int S, int n0, bool vec) {
 #pragma unroll
     for (int i = 0; i < kCT; ++i) {
-        const ulonglong2 q = P[i][lane], e = E[i][lane];
-        s.v[i][0] = fma2(f2{q.x}, s.v[i][0], f2{e.x});
-        s.v[i][1] = fma2(f2{q.y}, s.v[i][1], f2{e.y});
-    }
-}
-__device__ __forceinline__ void st_put(ulonglong2 (*d)[32], int lane, const St& s) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) d[i][lane] = make_ulonglong2(s.v[i][0].v, s.v[i][1].v);
-}
-__device__ __forceinline__ void st_get(St& s, const ulonglong2 (*d)[32], int lane) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) {
-        const ulonglong2 q = d[i][lane];
-        s.v[i][0].v = q.x;
-        s.v[i][1].v = q.y;
-    }
-}
-// States n0 .. n0 + 4 of features f and f + 1 of a (features, S) table; those
-// that do not exist read as 0 and are not written.
-__device__ __forceinline__ void st_load(St& s, const float* tab, int f, int nf, int S, int n0, bool vec) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) {
+        const int c = f + (i ^ swap);
         Vec<float, 4> r;
-        const int n = f + i < nf ? min(max(S - n0, 0), 4) : 0;
-        r.load_n(tab + static_cast<long long>(f + i) * S + n0, n, vec);
+        const int n = c < nf ? min(max(S - n0, 0), 4) : 0;
+        r.load_n(tab + static_cast<long long>(c) * S + n0, n, vec);
         s.v[i][0] = pk(r.get(0), r.get(1));
         s.v[i][1] = pk(r.get(2), r.get(3));
     }
 }
-__device__ __forceinline__ void st_store(const St& s, float* tab, int f, int nf, int S, int n0, bool vec) {
+__device__ __forceinline__ void st_store(const St& s, float* tab, int f, int swap, int nf, int S, int n0, bool vec) {
 #pragma unroll
     for (int i = 0; i < kCT; ++i) {
+        const int c = f + (i ^ swap);
         Vec<float, 4> r;
         float v[4];
         upk(s.v[i][0], v[0], v[1]);
         upk(s.v[i][1], v[2], v[3]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.set(j, v[j]);
-        const int n = f + i < nf ? min(max(S - n0, 0), 4) : 0;
-        r.store_n(tab + static_cast<long long>(f + i) * S + n0, n, vec);
+        const int n = c < nf ? min(max(S - n0, 0), 4) : 0;
+        r.store_n(tab + static_cast<long long>(c) * S + n0, n, vec);
     }
+}
+// h <- exp(A sum dt) h + E over one segment.
+__device__ __forceinline__ void st_chain(St& h, const ScanP& p, const St& A2, int b, int seg, int f, int swap, int nf, int n0) {
+    const long long row = static_cast<long long>(b) * p.nseg + seg;
+    St E;
+    st_load(E, p.seg_E + row * p.a.dim * p.a.nstate, f, swap, nf, p.a.nstate, n0, p.vec_n);
+#pragma unroll
+    for (int i = 0; i < kCT; ++i) {
+        const int c = f + (i ^ swap);
+        const float d = c < nf ? __ldg(p.seg_dt + row * p.a.dim + c) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) h.v[i][j] = fma2(ex22(mul2(pk(d, d), A2.v[i][j])), h.v[i][j], E.v[i][j]);
+    }
+}
+__device__ __forceinline__ void st_scale(St& s, float k) {
+#pragma unroll
+    for (int i = 0; i < kCT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s.v[i][j] = mul2(s.v[i][j], pk(k, k));
 }
 
 template <typename T, int NL>
@@ -126,8 +141,8 @@ inline void scan_params(ScanP& p, const sdtw_scan_args& a) {
     p.a = a;
     p.dg = a.dim / a.groups;
     p.tiles_g = (p.dg + K::CH - 1) / K::CH;
-    p.nchunk = (a.length + kScanChunk - 1) / kScanChunk;
-    const bool d = p.dg % K::VX == 0 && a.dim % K::VX == 0;
+    p.nchunk = (a.length + K::TS - 1) / K::TS;
+    const bool d = p.dg % K::VX == 0;
     const long long ds = a.dim;
     p.vec_x = d && vec_ok<T, K::VX>(a.x, a.x_batch, a.x_time);
     p.vec_delta = d && vec_ok<T, K::VX>(a.delta, a.delta_batch, a.delta_time);
@@ -145,16 +160,20 @@ inline void scan_params(ScanP& p, const sdtw_scan_args& a) {
               vec_ok<float, 4>(a.dstate_in, 0, 0) && vec_ok<float, 4>(a.dstate_out, 0, 0);
 }
 
-// Lanes over the states of a feature.
-inline int scan_lanes(int nstate) {
-    int nl = 1;
-    while (4 * nl < nstate) nl *= 2;
-    return nl;
+// The segments' tables at the start of a workspace, and their floats.
+inline size_t scan_segment_floats(int batch, int nseg, int dim, int nstate) {
+    return nseg > 1 ? static_cast<size_t>(batch) * nseg * dim * (nstate + 1) : 0;
+}
+inline void scan_segment_tables(ScanP& p, const ScanSplit& s, void* ws) {
+    p.nseg = s.nseg;
+    p.seglen = s.seglen;
+    // The states first: their 16-byte pieces stay aligned.
+    p.seg_E = static_cast<float*>(ws);
+    p.seg_dt = p.seg_E + static_cast<size_t>(p.a.batch) * s.nseg * p.a.dim * p.a.nstate;
 }
 
-template <int NL>
-inline long long scan_blocks(const ScanP& p) {
-    return static_cast<long long>(p.tiles_g) * p.a.groups * p.a.batch;
-}
+// The segments' first kernel: forward (u B added up) or backward over time
+// (gy C added up, with gy = dy or dy z sigmoid(z)).
+cudaError_t launch_scan_segments(const ScanP& p, bool reverse, cudaStream_t st);
 
 }  // namespace sdtw

@@ -10,17 +10,21 @@
 //   dA[n] += gh[n] a[n] h_prev[n] dt,          ddelta = (s + q x) softplus'(delta + bias)
 //   dx = q dt + gy D,   dD += gy x,            dz = dout y (sigmoid(z) (1 + z (1 - sigmoid(z))))
 //
-// A block walks over its chunks from the last to the first, from the states that
-// the forward stored at the chunks' starts.  As in the forward each warp keeps
-// the decays of its 8 steps in registers and runs the recurrence twice: from 0,
-// which gives the run's product P and end E, and with the states chained over
-// the warps; the reverse recurrence r has the same product P, so that both are
-// chained behind one barrier.  Every exponential is computed once.  The states
-// of the 8 steps stay in registers too (64 registers each for decays and states
-// per thread).  Sums over the states of a feature and over the features of dB
-// and dC are lane exchanges that halve the values at every step; what is left of
-// dB and dC per block goes to a partial table that a second kernel adds up in a
-// fixed order, so results do not change from call to call.
+// A warp walks over its staged pieces of TS steps from the last to the first,
+// from the states that the forward stored at their starts.  It runs 8 steps
+// forward, keeping their decays and states in registers (64 each per thread),
+// then the same 8 backward; the first half of a 16-step piece is run forward
+// once more in front of the second.  Reductions: the sums over the states of a
+// feature and over the features of dB and dC are lane exchanges that halve the
+// values at every step, mostly without selects, because the lanes hold their
+// two features, and their four states, in an order that depends on the lane
+// (two copies of dt, u and gy and four of B and C in shared memory provide it).
+// The 4 warps of a block take neighbouring features of one group, add up their
+// dB and dC in shared memory behind one barrier per piece, and share the staging
+// of B and C; what is left per block goes to a partial table that a second
+// kernel adds up in a fixed order, so results do not change from call to call.
+#include <algorithm>
+
 #include "selective_scan.cuh"
 
 namespace sdtw {
@@ -29,232 +33,313 @@ namespace {
 template <int NL>
 struct BwdSmem {
     using K = ScanTile<NL>;
-    float2 U[kScanWarps][kScanSteps][K::CH];  // (dt, u)
-    float G[kScanWarps][kScanSteps][K::CH];   // gy
-    float Q[kScanWarps][kScanSteps][K::CH], R[kScanWarps][kScanSteps][K::CH], Y[kScanWarps][kScanSteps][K::CH];
-    float B[kScanWarps][kScanSteps][K::NP], C[kScanWarps][kScanSteps][K::NP];
-    ulonglong2 P[2][kScanWarps][kCT][32], E[2][kScanWarps][kCT][32], R0[2][kScanWarps][kCT][32], carry[2][kCT][32];
+    static constexpr int NQ = K::CL < 4 ? K::CL : 4;  // copies of B and C: states permuted by n ^ q within fours
+    float4 U[kScanWarps][2][K::TS][K::CH / 2];        // (dt, u) of two features; copy 1 swapped
+    float2 G[kScanWarps][2][K::TS][K::CH / 2];        // gy
+    // Per element, for the last step of a piece: x, softplus', dout times the gate's derivative ...
+    float X[kScanWarps][K::TS][K::CH], D[kScanWarps][K::TS][K::CH], Z[kScanWarps][K::TS][K::CH];
+    // ... and the sums q, s and y.
+    float Q[kScanWarps][K::TS][K::CH], R[kScanWarps][K::TS][K::CH], Y[kScanWarps][K::TS][K::CH];
+    // One more row than steps, so that the copies start in different banks.
+    float B[2][NQ][K::TS + 1][K::NP], C[2][NQ][K::TS + 1][K::NP];
+    float acc[2][kScanWarps][K::TS][2][K::NP];  // the warps' dB, dC
 };
 
 template <typename T, int NL>
 __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanP p) {
     using K = ScanTile<NL>;
+    using M = BwdSmem<NL>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    BwdSmem<NL>& sm = *reinterpret_cast<BwdSmem<NL>*>(smem_raw);
-    const ScanPlace<NL> at(p);
+    M& sm = *reinterpret_cast<M*>(smem_raw);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nl = lane % NL, cl = lane / NL;
+    const int quads = (p.tiles_g + kScanWarps - 1) / kScanWarps;  // blocks over a group's features
+    const int gq = blockIdx.x % (quads * p.a.groups);
+    const int bs = blockIdx.x / (quads * p.a.groups);
+    const ScanPlace<NL> at(p, bs / p.nseg, bs % p.nseg, gq / quads, gq % quads * kScanWarps + w);
+    const int nl = lane % NL, cl = lane / NL, swap = nl & 1, n0 = nl * 4, perm = cl & (M::NQ - 1);
     const int S = p.a.nstate, L = p.a.length, dim = p.a.dim;
     const int len = seq_len(p.a.lengths, at.b, L);
     const int f0 = at.c0 + cl * kCT, fend = at.c0 + at.nc;
-    const int row = lane >> 2, col = (lane & 3) * K::VX, bcol = (lane & 3) * K::VN;
-    const int nx = min(max(at.nc - col, 0), K::VX), nb = min(max(S - bcol, 0), K::VN);
+    const int row = lane / K::LR, col = lane % K::LR * K::VX;
+    const int nx = min(max(at.nc - col, 0), K::VX);
+    // Staging of B and C: the block's 128 threads over TS rows.
+    constexpr int BR = kScanThreads / K::TS, BN = (K::NP + BR - 1) / BR;
+    const int brow = threadIdx.x / BR, bcol = threadIdx.x % BR * BN;
 
-    St A2, dA;
-    st_load(A2, p.a.A, f0, fend, S, nl * 4, p.vec_n);
+    St A2, dA, r;
+    st_load(A2, p.a.A, f0, swap, fend, S, n0, p.vec_n);
+    st_scale(A2, kL2e);
+    // States in this lane's order: register j holds state n0 + (j ^ perm).
+    auto permute = [&](St& s) {
 #pragma unroll
-    for (int i = 0; i < kCT; ++i)
+        for (int i = 0; i < kCT; ++i) {
+            float v[4], o[4];
+            upk(s.v[i][0], v[0], v[1]);
+            upk(s.v[i][1], v[2], v[3]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) A2.v[i][j] = mul2(A2.v[i][j], pk(kL2e, kL2e));
+            for (int j = 0; j < 4; ++j) {
+                const float a = perm & 1 ? v[j ^ 1] : v[j], b = perm & 1 ? v[j ^ 3] : v[j ^ 2];
+                o[j] = perm & 2 ? b : a;
+            }
+            s.v[i][0] = pk(o[0], o[1]);
+            s.v[i][1] = pk(o[2], o[3]);
+        }
+    };
+    permute(A2);
     st_set(dA, 0.f);
+    st_set(r, 0.f);
+    if (p.a.dstate_out) {
+        st_load(r, p.a.dstate_out + static_cast<long long>(at.b) * dim * S, f0, swap, fend, S, n0, p.vec_n);
+        permute(r);
+    }
+    if (p.nseg > 1) {
+        pdl_wait();
+        permute(A2);
+        permute(r);
+        for (int q = p.nseg - 1; q > at.seg; --q) st_chain(r, p, A2, at.b, q, f0, swap, fend, n0);
+        permute(A2);
+        permute(r);
+    }
     float dD[K::VX], dbias[K::VX];
 #pragma unroll
     for (int e = 0; e < K::VX; ++e) dD[e] = dbias[e] = 0.f;
-    if (w == 0) {
-        St r;
-        st_set(r, 0.f);
-        if (p.a.dstate_out) st_load(r, p.a.dstate_out + static_cast<long long>(at.b) * dim * S, f0, fend, S, nl * 4, p.vec_n);
-        st_put(sm.carry[0], lane, r);
-    }
     const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + at.c0 + col;
     const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0 + col;
     const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0 + col;
     const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + at.c0 + col;
-    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + at.g * p.a.B_group + bcol;
-    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + at.g * p.a.C_group + bcol;
+    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + at.g * p.a.B_group;
+    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + at.g * p.a.C_group;
+    const float* bias = p.a.delta_bias ? p.a.delta_bias + at.c0 + col : nullptr;
+    const float* skip = p.a.D ? p.a.D + at.c0 + col : nullptr;
     const long long out0 = static_cast<long long>(at.b) * L * dim + at.c0 + col;
 
-    const int nck = (len + kScanChunk - 1) / kScanChunk;
-    for (int ck = nck - 1; ck >= 0; --ck) {
-        const int buf = (nck - 1 - ck) & 1;
-        const int t = ck * kScanChunk + w * kScanSteps + row;  // the step that this lane stages
-        const bool in = t < len;
-        Vec<T, K::VX> rx, rd, rz, rg;
-        Vec<T, K::VN> rB, rC;
-        rx.load_n(xp + t * p.a.x_time, in ? nx : 0, p.vec_x);
-        rd.load_n(dp + t * p.a.delta_time, in ? nx : 0, p.vec_delta);
-        rg.load_n(gp + t * p.a.dy_time, in ? nx : 0, p.vec_dy);
-        if (p.a.z) rz.load_n(zp + t * p.a.z_time, in ? nx : 0, p.vec_z);
-        rB.load_n(Bp + t * p.a.B_time, in ? nb : 0, p.vec_B);
-        rC.load_n(Cp + t * p.a.C_time, in ? nb : 0, p.vec_C);
-        St hin;
-        st_load(hin, p.a.saved + (static_cast<long long>(at.b) * p.nchunk + ck) * dim * S, f0, fend, S, nl * 4, p.vec_n);
-        __syncwarp();
+    Vec<T, K::VX> rx, rd, rz, rg;
+    St h0;
+    auto fetch = [&](int tc) {
+        const int t = tc + row, n = t < len ? nx : 0;
+        rx.load_n(xp + t * p.a.x_time, n, p.vec_x);
+        rd.load_n(dp + t * p.a.delta_time, n, p.vec_delta);
+        rg.load_n(gp + t * p.a.dy_time, n, p.vec_dy);
+        if (p.a.z) rz.load_n(zp + t * p.a.z_time, n, p.vec_z);
+        st_load(h0, p.a.saved + (static_cast<long long>(at.b) * p.nchunk + tc / K::TS) * dim * S, f0, swap, fend, S, n0, p.vec_n);
+    };
+    auto stage_bc = [&](int buf, int tc) {
+        const int t = tc + brow;
 #pragma unroll
-        for (int e = 0; e < K::VX; ++e) {
-            float dt = rd.get(e) + (p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f);
-            if (p.a.softplus) dt = softplusf(dt);
-            if (!in) dt = 0.f;
-            float gy = rg.get(e);
-            if (p.a.z) {
-                const float z = rz.get(e);
-                gy *= z * sigmoidf(z);
+        for (int e = 0; e < BN; ++e) {
+            const int n = bcol + e;
+            if (n < K::NP) {
+                const bool in = t < len && n < S;
+                const float b = in ? to_f(Bp[t * p.a.B_time + n]) : 0.f, c = in ? to_f(Cp[t * p.a.C_time + n]) : 0.f;
+#pragma unroll
+                for (int q = 0; q < M::NQ; ++q) {
+                    sm.B[buf][q][brow][n ^ q] = b;
+                    sm.C[buf][q][brow][n ^ q] = c;
+                }
             }
-            sm.U[w][row][col + e] = make_float2(dt, dt * rx.get(e));
-            sm.G[w][row][col + e] = gy;
         }
+    };
+    // The block's dB, dC of a piece.
+    auto put_bc = [&](int buf, int tc) {
+        float* d = p.part_bc + ((static_cast<long long>(gq) * p.a.batch + at.b) * L + tc) * 2 * K::NP;
+        const int rows = min(K::TS, min(at.t1, len) - tc);
+        for (int i = threadIdx.x; i < rows * 2 * K::NP; i += kScanThreads) {
+            float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < K::VN; ++e) {
-            sm.B[w][row][bcol + e] = rB.get(e);
-            sm.C[w][row][bcol + e] = rC.get(e);
+            for (int q = 0; q < kScanWarps; ++q) s += (&sm.acc[buf][q][0][0][0])[i];
+            d[i] = s;
         }
-        __syncwarp();
+    };
 
-        f2 a[kScanSteps][kCT][2], h[kScanSteps][kCT][2];
-        St P, E;
-        st_set(E, 0.f);
-        st_set(P, 1.f);
+    const int tend = min(at.t1, len), pieces = tend > at.t0 ? (tend - at.t0 + K::TS - 1) / K::TS : 0;
+    if (pieces > 0) {
+        fetch(at.t0 + (pieces - 1) * K::TS);
+        stage_bc(0, at.t0 + (pieces - 1) * K::TS);
+    }
+    for (int k = 0; k < pieces; ++k) {
+        const int tc = at.t0 + (pieces - 1 - k) * K::TS, buf = k & 1, t = tc + row;
+        const bool in = t < len;
+        St hs = h0;
+        __syncwarp();
 #pragma unroll
-        for (int s = 0; s < kScanSteps; ++s) {
-            const float4 du = *reinterpret_cast<const float4*>(&sm.U[w][s][cl * kCT]);
-            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[w][s][nl * 4]);
+        for (int e = 0; e < K::VX; e += 2) {
+            float dt[2], u[2], g[2];
 #pragma unroll
-            for (int i = 0; i < kCT; ++i) {
-                const float dt = i ? du.z : du.x, u = i ? du.w : du.y;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    a[s][i][j] = ex22(mul2(pk(dt, dt), A2.v[i][j]));
-                    E.v[i][j] = fma2(a[s][i][j], E.v[i][j], mul2(pk(u, u), f2{j ? bv.y : bv.x}));
-                    h[s][i][j] = E.v[i][j];
-                    P.v[i][j] = mul2(P.v[i][j], a[s][i][j]);
+            for (int i = 0; i < 2; ++i) {
+                const float x = rx.get(e + i);
+                float ds = 1.f, zf = 0.f;
+                dt[i] = rd.get(e + i) + (bias && e + i < nx ? __ldg(bias + e + i) : 0.f);
+                if (p.a.softplus) dt[i] = softplusf(dt[i], &ds);
+                if (!in) dt[i] = ds = 0.f;
+                g[i] = rg.get(e + i);
+                if (p.a.z) {
+                    const float z = rz.get(e + i), sg = sigmoidf(z);
+                    zf = g[i] * sg * fmaf(z, 1.f - sg, 1.f);
+                    g[i] *= z * sg;
                 }
+                u[i] = dt[i] * x;
+                sm.X[w][row][col + e + i] = x;
+                sm.D[w][row][col + e + i] = ds;
+                sm.Z[w][row][col + e + i] = zf;
             }
+            sm.U[w][0][row][(col + e) / 2] = make_float4(dt[0], u[0], dt[1], u[1]);
+            sm.U[w][1][row][(col + e) / 2] = make_float4(dt[1], u[1], dt[0], u[0]);
+            sm.G[w][0][row][(col + e) / 2] = make_float2(g[0], g[1]);
+            sm.G[w][1][row][(col + e) / 2] = make_float2(g[1], g[0]);
         }
-        st_put(sm.P[buf][w], lane, P);
-        st_put(sm.E[buf][w], lane, E);
-        St r;
-        st_set(r, 0.f);
+        // Behind this barrier: B and C of this piece, and the warps' dB and dC
+        // of the one before.  The buffers alternate, so one barrier is enough.
+        __syncthreads();
+        if (k > 0) put_bc(buf ^ 1, tc + K::TS);
+        permute(hs);
+
+        f2 a[kRun][kCT][2], h[kRun][kCT][2];
+        // 8 steps forward from hs; `keep` stores the decays and the states.
+        auto forward = [&](int sb, St& s0, bool keep) {
 #pragma unroll
-        for (int s = kScanSteps - 1; s >= 0; --s) {
-            const float2 gy = *reinterpret_cast<const float2*>(&sm.G[w][s][cl * kCT]);
-            const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sm.C[w][s][nl * 4]);
+            for (int s = 0; s < kRun; ++s) {
+                const float4 du = sm.U[w][swap][sb + s][cl];
+                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][perm][sb + s][n0]);
 #pragma unroll
-            for (int i = 0; i < kCT; ++i) {
-                const float g = i ? gy.y : gy.x;
+                for (int i = 0; i < kCT; ++i) {
+                    const float dt = i ? du.z : du.x, u = i ? du.w : du.y;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) r.v[i][j] = mul2(a[s][i][j], fma2(pk(g, g), f2{j ? cv.y : cv.x}, r.v[i][j]));
-            }
-        }
-        st_put(sm.R0[buf][w], lane, r);
-        __syncthreads();  // one per chunk: the buffers alternate
-        for (int q = 0; q < w; ++q) st_chain(hin, sm.P[buf][q], sm.E[buf][q], lane);
-        st_get(r, sm.carry[buf], lane);
-        for (int q = kScanWarps - 1; q > w; --q) st_chain(r, sm.P[buf][q], sm.R0[buf][q], lane);
-        if (w == 0) {
-            St c = r;
-            st_chain(c, sm.P[buf][0], sm.R0[buf][0], lane);
-            st_put(sm.carry[buf ^ 1], lane, c);
-        }
-        // The states from the true start: h = (h from 0) + (product of decays) hin.
-        St pc = hin;
-#pragma unroll
-        for (int s = 0; s < kScanSteps; ++s)
-#pragma unroll
-            for (int i = 0; i < kCT; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    pc.v[i][j] = mul2(pc.v[i][j], a[s][i][j]);
-                    h[s][i][j] = add2(h[s][i][j], pc.v[i][j]);
-                }
-        using SumF = LaneSum<2 * kCT, 1, NL>;      // over the states of a feature, 2 steps at a time
-        using SumN = LaneSum<8, NL, 32 / NL>;      // over the features: 4 states of dB, 4 of dC
-        float vq[2 * kCT], vr[2 * kCT], vy[2 * kCT];
-#pragma unroll
-        for (int s = kScanSteps - 1; s >= 0; --s) {
-            const float4 du = *reinterpret_cast<const float4*>(&sm.U[w][s][cl * kCT]);
-            const float2 gy = *reinterpret_cast<const float2*>(&sm.G[w][s][cl * kCT]);
-            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[w][s][nl * 4]);
-            const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sm.C[w][s][nl * 4]);
-            f2 aB[2], aC[2];
-#pragma unroll
-            for (int i = 0; i < kCT; ++i) {
-                const float dt = i ? du.z : du.x, u = i ? du.w : du.y, g = i ? gy.y : gy.x;
-                f2 q, sa, y;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const f2 b2{j ? bv.y : bv.x}, c2{j ? cv.y : cv.x};
-                    const f2 gh = fma2(pk(g, g), c2, r.v[i][j]);
-                    r.v[i][j] = mul2(a[s][i][j], gh);
-                    const f2 hp = s > 0 ? h[s > 0 ? s - 1 : 0][i][j] : hin.v[i][j];
-                    const f2 k = mul2(r.v[i][j], hp);
-                    dA.v[i][j] = fma2(pk(dt, dt), k, dA.v[i][j]);
-                    aC[j] = i ? fma2(pk(g, g), h[s][i][j], aC[j]) : mul2(pk(g, g), h[s][i][j]);
-                    aB[j] = i ? fma2(pk(u, u), gh, aB[j]) : mul2(pk(u, u), gh);
-                    q = j ? fma2(gh, b2, q) : mul2(gh, b2);
-                    sa = j ? fma2(k, A2.v[i][j], sa) : mul2(k, A2.v[i][j]);
-                    y = j ? fma2(c2, h[s][i][j], y) : mul2(c2, h[s][i][j]);
-                }
-                vq[(s & 1) * kCT + i] = sum2(q);
-                vr[(s & 1) * kCT + i] = sum2(sa);
-                vy[(s & 1) * kCT + i] = sum2(y);
-            }
-            float v[8];
-            upk(aB[0], v[0], v[1]);
-            upk(aB[1], v[2], v[3]);
-            upk(aC[0], v[4], v[5]);
-            upk(aC[1], v[6], v[7]);
-            SumN::run(v, lane);
-            const int ts = ck * kScanChunk + w * kScanSteps + s;
-            if (ts < len && SumN::owner(lane)) {
-                const int k0 = SumN::slot(lane);  // 0-3: dB, 4-7: dC
-                float* d = p.part_bc +
-                           ((static_cast<long long>(at.tile) * p.a.batch + at.b) * L + ts) * 2 * K::NP + (k0 / 4) * K::NP + nl * 4 + k0 % 4;
-#pragma unroll
-                for (int k = 0; k < SumN::kept; ++k) d[k % 4 + k / 4 * K::NP] = v[k];
-            }
-            if ((s & 1) == 0) {
-                SumF::run(vq, lane);
-                SumF::run(vr, lane);
-                SumF::run(vy, lane);
-                if (SumF::owner(lane)) {
-                    const int slot = SumF::slot(lane);
-#pragma unroll
-                    for (int k = 0; k < SumF::kept; ++k) {
-                        const int ss = s + (slot + k) / kCT, c = cl * kCT + (slot + k) % kCT;
-                        sm.Q[w][ss][c] = vq[k];
-                        sm.R[w][ss][c] = vr[k];
-                        sm.Y[w][ss][c] = vy[k];
+                    for (int j = 0; j < 2; ++j) {
+                        const f2 d = ex22(mul2(pk(dt, dt), A2.v[i][j]));
+                        s0.v[i][j] = fma2(d, s0.v[i][j], mul2(pk(u, u), f2{j ? bv.y : bv.x}));
+                        if (keep) {
+                            a[s][i][j] = d;
+                            h[s][i][j] = s0.v[i][j];
+                        }
                     }
                 }
             }
+        };
+        St hm = hs;
+        if constexpr (K::TS > kRun) forward(0, hm, false);
+#pragma unroll 1
+        for (int sb = K::TS - kRun; sb >= 0; sb -= kRun) {
+            St hin;
+#pragma unroll
+            for (int i = 0; i < kCT; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) hin.v[i][j].v = sb > 0 ? hm.v[i][j].v : hs.v[i][j].v;
+            St run = hin;
+            forward(sb, run, true);
+            float vq[2 * kCT], vr[2 * kCT], vy[2 * kCT];
+#pragma unroll
+            for (int s = kRun - 1; s >= 0; --s) {
+                const float4 du = sm.U[w][swap][sb + s][cl];
+                const float2 gy = sm.G[w][swap][sb + s][cl];
+                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][perm][sb + s][n0]);
+                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sm.C[buf][perm][sb + s][n0]);
+                f2 aB[2], aC[2];
+#pragma unroll
+                for (int i = 0; i < kCT; ++i) {
+                    const float dt = i ? du.z : du.x, u = i ? du.w : du.y, g = i ? gy.y : gy.x;
+                    f2 q, sa, y;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const f2 b2{j ? bv.y : bv.x}, c2{j ? cv.y : cv.x};
+                        const f2 gh = fma2(pk(g, g), c2, r.v[i][j]);
+                        r.v[i][j] = mul2(a[s][i][j], gh);
+                        const f2 hp = s > 0 ? h[s > 0 ? s - 1 : 0][i][j] : hin.v[i][j];
+                        const f2 kk = mul2(r.v[i][j], hp);
+                        dA.v[i][j] = fma2(pk(dt, dt), kk, dA.v[i][j]);
+                        aC[j] = i ? fma2(pk(g, g), h[s][i][j], aC[j]) : mul2(pk(g, g), h[s][i][j]);
+                        aB[j] = i ? fma2(pk(u, u), gh, aB[j]) : mul2(pk(u, u), gh);
+                        q = j ? fma2(gh, b2, q) : mul2(gh, b2);
+                        sa = j ? fma2(kk, A2.v[i][j], sa) : mul2(kk, A2.v[i][j]);
+                        y = j ? fma2(c2, h[s][i][j], y) : mul2(c2, h[s][i][j]);
+                    }
+                    // Pairs of registers (step of an even pair, feature): see pair_exchange.
+                    vq[(s & 1) * kCT + i] = sum2(q);
+                    vr[(s & 1) * kCT + i] = sum2(sa);
+                    vy[(s & 1) * kCT + i] = sum2(y);
+                }
+                // dB, dC over the lanes' features: register j is state n0 + (j ^ perm).
+                float vb[4], vc[4];
+                upk(aB[0], vb[0], vb[1]);
+                upk(aB[1], vb[2], vb[3]);
+                upk(aC[0], vc[0], vc[1]);
+                upk(aC[1], vc[2], vc[3]);
+                float* acc = &sm.acc[buf][w][sb + s][0][n0];
+                if constexpr (M::NQ == 4) {
+                    float b1[2], c1[2], b0[1], c0[1];
+                    pair_exchange(vb, b1, NL);  // state bit 0
+                    pair_exchange(vc, c1, NL);
+                    pair_exchange(b1, b0, 2 * NL);  // state bit 1
+                    pair_exchange(c1, c0, 2 * NL);
+                    // dB to the lanes without bit 4 NL, dC to those with it (none for 8 lanes per feature: both).
+                    if constexpr (K::CL >= 8) {
+                        const bool up = lane & (4 * NL);
+                        float v = (up ? c0[0] : b0[0]) + __shfl_xor_sync(0xffffffffu, up ? b0[0] : c0[0], 4 * NL);
+#pragma unroll
+                        for (int m = 8 * NL; m < 32; m *= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+                        if (lane < 8 * NL) acc[(up ? K::NP : 0) + perm] = v;
+                    } else {
+                        acc[perm] = b0[0];
+                        acc[K::NP + perm] = c0[0];
+                    }
+                } else {  // two lane groups: state bit 0 only
+                    float b1[2], c1[2];
+                    pair_exchange(vb, b1, NL);
+                    pair_exchange(vc, c1, NL);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        acc[2 * j + perm] = b1[j];
+                        acc[K::NP + 2 * j + perm] = c1[j];
+                    }
+                }
+                if ((s & 1) == 0) {  // q, s, y over the lanes' states, two steps at a time
+                    auto put = [&](float(&v)[2 * kCT], float (*out)[K::CH]) {
+                        if constexpr (NL == 1) {
+#pragma unroll
+                            for (int i = 0; i < 2 * kCT; ++i) out[sb + s + i / kCT][cl * kCT + i % kCT] = v[i];
+                        } else {
+                            float o[2];
+                            pair_exchange(v, o, 1);
+                            using Sum = LaneSum<2, 2, NL / 2>;
+                            Sum::run(o, lane);
+                            if (Sum::owner(lane)) {
+                                const int slot = Sum::slot(lane);
+#pragma unroll
+                                for (int i = 0; i < Sum::kept; ++i) out[sb + s + slot + i][cl * kCT + swap] = o[i];
+                            }
+                        }
+                    };
+                    put(vq, sm.Q[w]);
+                    put(vr, sm.R[w]);
+                    put(vy, sm.Y[w]);
+                }
+            }
+        }
+        if (k + 1 < pieces) {  // on their way during what follows
+            fetch(tc - K::TS);
+            stage_bc(buf ^ 1, tc - K::TS);
         }
         __syncwarp();
         Vec<T, K::VX> ox, od, oz;
 #pragma unroll
         for (int e = 0; e < K::VX; ++e) {
-            const float dt = sm.U[w][row][col + e].x, gy = sm.G[w][row][col + e], q = sm.Q[w][row][col + e];
-            const float x = rx.get(e);
-            const float Df = p.a.D && e < nx ? __ldg(p.a.D + at.c0 + col + e) : 0.f;
-            float dd = fmaf(q, x, kLn2 * sm.R[w][row][col + e]);
-            if (p.a.softplus) dd *= sigmoidf(rd.get(e) + (p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f));
-            if (!in) dd = 0.f;
+            const float2 du = reinterpret_cast<const float2*>(sm.U[w][0][row])[col + e];
+            const float gy = reinterpret_cast<const float*>(sm.G[w][0][row])[col + e];
+            const float q = sm.Q[w][row][col + e], x = sm.X[w][row][col + e];
+            const float Df = skip && e < nx ? __ldg(skip + e) : 0.f;
+            const float dd = fmaf(q, x, kLn2 * sm.R[w][row][col + e]) * sm.D[w][row][col + e];
             dbias[e] += dd;
             dD[e] = fmaf(gy, x, dD[e]);
-            ox.set(e, fmaf(q, dt, gy * Df));
+            ox.set(e, fmaf(q, du.x, gy * Df));
             od.set(e, dd);
-            if (p.a.z) {
-                const float z = rz.get(e), sg = sigmoidf(z);
-                const float y = fmaf(Df, x, sm.Y[w][row][col + e]);
-                oz.set(e, rg.get(e) * y * (sg * (1.f + z * (1.f - sg))));
-            }
+            oz.set(e, sm.Z[w][row][col + e] * fmaf(Df, x, sm.Y[w][row][col + e]));
         }
-        const int no = t < L ? nx : 0;
+        const int no = t < at.t1 ? nx : 0;
         const long long o = out0 + static_cast<long long>(t) * dim;
         if (p.a.dx) ox.store_n(static_cast<T*>(p.a.dx) + o, no, p.vec_dx);
         if (p.a.ddelta) od.store_n(static_cast<T*>(p.a.ddelta) + o, no, p.vec_ddelta);
         if (p.a.z && p.a.dz) oz.store_n(static_cast<T*>(p.a.dz) + o, no, p.vec_dz);
     }
-    for (int t = nck * kScanChunk + w * kScanSteps + row; t < L; t += kScanChunk) {
+    for (int t = at.t0 + pieces * K::TS + row; t < at.t1; t += K::TS) {
         Vec<T, K::VX> o;
         o.zero();
         const long long at_t = out0 + static_cast<long long>(t) * dim;
@@ -263,57 +348,33 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const ScanP p
         if (p.a.z && p.a.dz) o.store_n(static_cast<T*>(p.a.dz) + at_t, nx, p.vec_dz);
     }
     __syncthreads();
-    if (w == 0 && p.a.dstate_in) {
-        St r;
-        st_get(r, sm.carry[nck & 1], lane);
-        st_store(r, p.a.dstate_in + static_cast<long long>(at.b) * dim * S, f0, fend, S, nl * 4, p.vec_n);
-    }
-    // This batch entry's dA, dD and ddelta_bias: the warps' sums in a fixed order.
-    float* par = p.part_par + static_cast<long long>(at.b) * dim * (S + 2);
-    st_put(sm.P[0][w], lane, dA);
+    if (pieces > 0) put_bc((pieces - 1) & 1, at.t0);
+    permute(dA);
+    permute(r);
+    if (at.seg == 0 && p.a.dstate_in)
+        st_store(r, p.a.dstate_in + static_cast<long long>(at.b) * dim * S, f0, swap, fend, S, n0, p.vec_n);
+    // The segment's dA, dD and ddelta_bias.
+    float* par = p.part_par + (static_cast<long long>(at.b) * p.nseg + at.seg) * dim * (S + 2);
+    st_store(dA, par, f0, swap, fend, S, n0, p.vec_n && dim % 2 == 0);
 #pragma unroll
     for (int e = 0; e < K::VX; ++e) {
 #pragma unroll
-        for (int m = 4; m < 32; m *= 2) {
+        for (int m = K::LR; m < 32; m *= 2) {
             dD[e] += __shfl_xor_sync(0xffffffffu, dD[e], m);
             dbias[e] += __shfl_xor_sync(0xffffffffu, dbias[e], m);
         }
-        if (row == 0) {
-            sm.Q[w][0][col + e] = dD[e];
-            sm.R[w][0][col + e] = dbias[e];
-        }
-    }
-    __syncthreads();
-    if (w == 0) {
-#pragma unroll
-        for (int q = 1; q < kScanWarps; ++q) {
-            St o;
-            st_get(o, sm.P[0][q], lane);
-#pragma unroll
-            for (int i = 0; i < kCT; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) dA.v[i][j] = add2(dA.v[i][j], o.v[i][j]);
-        }
-        st_store(dA, par, f0, fend, S, nl * 4, p.vec_n && dim % 2 == 0);
-    } else if (w == 1) {
-        for (int c = lane; c < at.nc; c += 32) {
-            float d = 0.f, s = 0.f;
-#pragma unroll
-            for (int q = 0; q < kScanWarps; ++q) {
-                d += sm.Q[q][0][c];
-                s += sm.R[q][0][c];
-            }
-            par[static_cast<long long>(dim) * S + at.c0 + c] = d;
-            par[static_cast<long long>(dim) * (S + 1) + at.c0 + c] = s;
+        if (row == 0 && e < nx) {
+            par[static_cast<long long>(dim) * S + at.c0 + col + e] = dD[e];
+            par[static_cast<long long>(dim) * (S + 1) + at.c0 + col + e] = dbias[e];
         }
     }
 }
 
 // Adds the partial sums in a fixed order: blocks below nbc one element of dB or
-// dC per thread (over the group's tiles), the others one of dA, dD and
-// ddelta_bias (over the batch).
+// dC per thread (over the group's blocks of features), the others one of dA, dD
+// and ddelta_bias (over the batch and its segments).
 template <typename T>
-__global__ void __launch_bounds__(256) scan_sum_kernel(const ScanP p, long long nbc, int NP) {
+__global__ void __launch_bounds__(256) scan_sum_kernel(const ScanP p, long long nbc, int NP, int quads) {
     pdl_wait();
     const int S = p.a.nstate, G = p.a.groups, dim = p.a.dim, L = p.a.length;
     if (blockIdx.x < nbc) {
@@ -328,10 +389,10 @@ __global__ void __launch_bounds__(256) scan_sum_kernel(const ScanP p, long long 
         if (!out) return;
         float s = 0.f;
         if (t < seq_len(p.a.lengths, b, L)) {
-            const long long tile = static_cast<long long>(p.a.batch) * L * 2 * NP;
-            const float* q = p.part_bc + g * p.tiles_g * tile + bt * 2 * NP + which * NP + n;
+            const long long part = static_cast<long long>(p.a.batch) * L * 2 * NP;
+            const float* q = p.part_bc + g * quads * part + bt * 2 * NP + which * NP + n;
 #pragma unroll 8
-            for (int k = 0; k < p.tiles_g; ++k) s += q[k * tile];
+            for (int k = 0; k < quads; ++k) s += q[k * part];
         }
         static_cast<T*>(out)[rowg * S + n] = from_f<T>(s);
         return;
@@ -339,8 +400,9 @@ __global__ void __launch_bounds__(256) scan_sum_kernel(const ScanP p, long long 
     const long long i = (blockIdx.x - nbc) * 256 + threadIdx.x, cols = static_cast<long long>(dim) * (S + 2);
     if (i >= cols) return;
     float s = 0.f;
+    const int rows = p.a.batch * p.nseg;
 #pragma unroll 8
-    for (int b = 0; b < p.a.batch; ++b) s += p.part_par[b * cols + i];
+    for (int b = 0; b < rows; ++b) s += p.part_par[b * cols + i];
     const long long dA = static_cast<long long>(dim) * S;
     if (i < dA) {
         if (p.a.dA) p.a.dA[i] = s;
@@ -351,28 +413,36 @@ __global__ void __launch_bounds__(256) scan_sum_kernel(const ScanP p, long long 
     }
 }
 
-size_t bc_floats(int batch, int length, int dim, int groups, int nstate) {
-    const int nl = scan_lanes(nstate), ch = 32 / nl * kCT, dg = dim / groups;
-    return static_cast<size_t>(groups) * ((dg + ch - 1) / ch) * batch * length * 2 * 4 * nl;
+int scan_quads(int dim, int groups, int nstate) {
+    const int ch = 32 / scan_lanes(nstate) * kCT * kScanWarps;
+    return (dim / groups + ch - 1) / ch;
 }
+size_t bc_floats(int batch, int length, int dim, int groups, int nstate) {
+    return static_cast<size_t>(groups) * scan_quads(dim, groups, nstate) * batch * length * 2 * 4 * scan_lanes(nstate);
+}
+size_t up4(size_t n) { return (n + 3) / 4 * 4; }  // whole 16-byte pieces
 
 template <typename T, int NL>
 cudaError_t run_scan_bwd(const sdtw_scan_args& a, cudaStream_t st) {
     ScanP p{};
     scan_params<T, NL>(p, a);
+    const ScanSplit split = scan_split(a.batch, a.length, a.dim, a.groups, a.nstate, true);
     p.part_bc = static_cast<float*>(a.workspace);
-    p.part_par = p.part_bc + bc_floats(a.batch, a.length, a.dim, a.groups, a.nstate);
-    const long long blocks = scan_blocks<NL>(p);
+    float* seg = p.part_bc + bc_floats(a.batch, a.length, a.dim, a.groups, a.nstate);
+    scan_segment_tables(p, split, seg);
+    p.part_par = seg + up4(scan_segment_floats(a.batch, split.nseg, a.dim, a.nstate));
+    const int quads = scan_quads(a.dim, a.groups, a.nstate);
+    const long long blocks = static_cast<long long>(quads) * a.groups * a.batch * p.nseg;
     const long long nbc = (static_cast<long long>(a.batch) * a.length * a.groups * 2 * 4 * NL + 255) / 256;
     const long long npar = (static_cast<long long>(a.dim) * (a.nstate + 2) + 255) / 256;
     if (blocks > 0x7fffffffll || nbc + npar > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     const int smem = static_cast<int>(sizeof(BwdSmem<NL>));
     cudaError_t e = cudaFuncSetAttribute(scan_bwd_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    scan_bwd_kernel<T, NL><<<static_cast<unsigned>(blocks), kScanThreads, smem, st>>>(p);
-    e = cudaGetLastError();
+    if (p.nseg > 1 && (e = launch_scan_segments(p, true, st)) != cudaSuccess) return e;
+    e = launch_pdl(p.nseg > 1, scan_bwd_kernel<T, NL>, dim3(static_cast<unsigned>(blocks)), dim3(kScanThreads), smem, st, p);
     if (e != cudaSuccess) return e;
-    return launch_pdl(true, scan_sum_kernel<T>, dim3(static_cast<unsigned>(nbc + npar)), dim3(256), 0, st, p, nbc, 4 * NL);
+    return launch_pdl(true, scan_sum_kernel<T>, dim3(static_cast<unsigned>(nbc + npar)), dim3(256), 0, st, p, nbc, 4 * NL, quads);
 }
 
 template <typename T>
@@ -389,7 +459,10 @@ cudaError_t run_scan_bwd_t(const sdtw_scan_args& a, cudaStream_t st) {
 }  // namespace
 
 size_t scan_bwd_ws(int batch, int length, int dim, int groups, int nstate) {
-    return (bc_floats(batch, length, dim, groups, nstate) + static_cast<size_t>(batch) * dim * (nstate + 2)) * sizeof(float);
+    const int nseg = scan_split(batch, length, dim, groups, nstate, true).nseg;
+    return (bc_floats(batch, length, dim, groups, nstate) + up4(scan_segment_floats(batch, nseg, dim, nstate)) +
+            static_cast<size_t>(batch) * nseg * dim * (nstate + 2)) *
+           sizeof(float);
 }
 
 cudaError_t launch_scan_bwd(const sdtw_scan_args& a, cudaStream_t st) {

@@ -147,9 +147,35 @@ inline bool vec_ok(const void* p, long long s0, long long s1, long long s2 = 0) 
 
 // Logistic function: 1 / (1 + exp(-v)).  exp(-v) overflows to infinity below
 // v = -88.7, where the quotient is 0 as it should be.
-__device__ __forceinline__ float sigmoidf(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-// log(1 + exp(v)) without overflow, and without losing exp(v) next to 1.
-__device__ __forceinline__ float softplusf(float v) { return fmaxf(v, 0.f) + log1pf(__expf(-fabsf(v))); }
+__device__ __forceinline__ float sigmoidf(float v) { return rcpf(1.f + ex2f(-1.4426950408889634f * v)); }
+// Derivative of v sigmoid(v).
+__device__ __forceinline__ float dsilu(float v) {
+    const float sg = sigmoidf(v);
+    return sg * fmaf(v, 1.f - sg, 1.f);
+}
+
+// softplus(v) = log(1 + exp(v)) = max(v, 0) + log1p(e) with e = exp(-|v|), and
+// its derivative, the logistic function, from the same e.
+//   e      2^t with t = -|v| log2(e) rounded, times 1 + (what t lost) ln 2: the
+//          rounding of t alone would cost |v| 2^-24 of every step size
+//   log1p  2 atanh(s), s = e / (2 + e) in (0, 1/3], with atanh(s) = s P(s^2) and
+//          P of degree 5 fitted at Chebyshev nodes (1e-10); no small difference
+//          of near-equal numbers, so tiny step sizes keep their relative accuracy
+__device__ __forceinline__ float softplusf(float v, float* deriv = nullptr) {
+    const float n = -fabsf(v);
+    const float t = n * 1.44269502f;
+    const float lost = fmaf(n, 1.92596303e-8f, fmaf(n, 1.44269502f, -t));
+    float e = ex2f(t);
+    e = fmaf(e, lost * 0.693147181f, e);
+    const float s = e * rcpf(2.f + e), z = s * s;
+    float q = fmaf(z, 0.122047015f, 0.106971338f);
+    q = fmaf(z, q, 0.143103123f);
+    q = fmaf(z, q, 0.199993476f);
+    q = fmaf(z, q, 0.333333403f);
+    q = fmaf(z, q, 1.f);
+    if (deriv) *deriv = (v >= 0.f ? 1.f : e) * rcpf(1.f + e);
+    return fmaf(2.f * s, q, fmaxf(v, 0.f));
+}
 
 // Packed float32 pairs: halves the instructions of multiplies and adds.
 struct f2 {
@@ -239,6 +265,15 @@ struct LaneSum {
         return own;
     }
 };
+
+// One halving exchange over lane bit m of values whose pairs (2k, 2k + 1) are
+// stored swapped in the lanes with that bit set: every lane keeps the even
+// registers and sends the odd ones, without selects.
+template <int K>
+__device__ __forceinline__ void pair_exchange(const float (&v)[K], float (&out)[K / 2], int m) {
+#pragma unroll
+    for (int k = 0; k < K / 2; ++k) out[k] = v[2 * k] + __shfl_xor_sync(0xffffffffu, v[2 * k + 1], m);
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -23,11 +23,24 @@ size_t conv_bwd_ws(int batch, int length, int dim, int width);
 
 // selective_scan_fwd.cu, selective_scan_bwd.cu
 constexpr int kScanMaxState = 64;
-constexpr int kScanChunk = 32;  // time steps between two stored states
+// Lanes over the states of a feature (4 states each).
+constexpr int scan_lanes(int nstate) {
+    int nl = 1;
+    while (4 * nl < nstate) nl *= 2;
+    return nl;
+}
+// Time steps staged at a time, which are also those between two stored states:
+// 16, or 8 for up to 8 states, whose tiles have more features.
+constexpr int scan_stage_steps(int lanes) { return lanes >= 4 ? 16 : 8; }
+struct ScanSplit {
+    int nseg, seglen;
+};
+ScanSplit scan_split(int batch, int length, int dim, int groups, int nstate, bool backward);
 cudaError_t launch_scan_fwd(const sdtw_scan_args& a, cudaStream_t st);
 cudaError_t launch_scan_bwd(const sdtw_scan_args& a, cudaStream_t st);
 cudaError_t launch_scan_step(const sdtw_scan_args& a, cudaStream_t st);
 size_t scan_states(int batch, int length, int dim, int nstate);
+size_t scan_fwd_ws(int batch, int length, int dim, int groups, int nstate);
 size_t scan_bwd_ws(int batch, int length, int dim, int groups, int nstate);
 
 }  // namespace sdtw

@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -76,6 +77,7 @@ _SIGS = {
     "sdtw_conv_backward": ([_P, _P], _I),
     "sdtw_conv_step": ([_P, _P], _I),
     "sdtw_scan_saved_elems": ([_I, _I, _I, _I], _SZ),
+    "sdtw_scan_forward_workspace_bytes": ([_I, _I, _I, _I, _I], _SZ),
     "sdtw_scan_workspace_bytes": ([_I, _I, _I, _I, _I], _SZ),
     "sdtw_scan_forward": ([_P, _P], _I),
     "sdtw_scan_backward": ([_P, _P], _I),
@@ -648,29 +650,40 @@ def cpu_backward(R: torch.Tensor, grad_out: torch.Tensor | None, gamma: float, b
 
 
 # ----------------------------------------------------------------------------- sequence operators
-# Argument blocks of include/sdtw_b200.h, field for field.
+# Argument blocks of include/sdtw_b200.h, field for field: a ctypes Structure,
+# and the same layout as a struct.Struct.  Calls use the latter: a single new
+# time step is a call of a few microseconds, and filling a Structure field by
+# field costs as much again.
+_KINDS = {"i": ("i", ctypes.c_int), "l": ("q", ctypes.c_longlong), "f": ("f", ctypes.c_float),
+          "p": ("P", ctypes.c_void_p), "z": ("N", ctypes.c_size_t)}
+
+
 def _block(name: str, spec: str):
-    kinds = {"i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "p": ctypes.c_void_p, "z": ctypes.c_size_t}
-    fields = [(f, kinds[kind]) for kind, names in (part.split(":") for part in spec.split()) for f in names.split(",")]
-    return type(name, (ctypes.Structure,), {"_fields_": fields})
+    fields = [(f, kind) for kind, names in (part.split(":") for part in spec.split()) for f in names.split(",")]
+    cls = type(name, (ctypes.Structure,), {"_fields_": [(f, _KINDS[k][1]) for f, k in fields]})
+    return cls, struct.Struct("@" + "".join(_KINDS[k][0] for _, k in fields)).pack
 
 
-LayerNormArgs = _block("LayerNormArgs", "i:dtype,dim l:rows f:eps p:x l:x_stride p:weight,bias,y,mean,rstd,dy "
-                                        "l:dy_stride p:dx,dweight,dbias,workspace z:workspace_bytes")
-ConvArgs = _block("ConvArgs", "i:dtype,batch,length,dim,width,silu p:x l:x_batch,x_time p:weight,bias,lengths,state_in "
-                              "l:state_in_batch p:state_out l:state_out_batch p:y,dy l:dy_batch,dy_time "
-                              "p:dstate_out,dx,dstate_in,dweight,dbias,workspace z:workspace_bytes")
-ScanArgs = _block("ScanArgs", "i:dtype,batch,length,dim,groups,nstate,softplus p:x,delta,z "
-                              "l:x_batch,x_time,delta_batch,delta_time,z_batch,z_time p:B,C "
-                              "l:B_batch,B_time,B_group,C_batch,C_time,C_group p:A,D,delta_bias,lengths,state_in "
-                              "l:state_in_batch p:state_out l:state_out_batch p:saved,y,dy l:dy_batch,dy_time "
-                              "p:dstate_out,dx,ddelta,dz,dB,dC,dA,dD,ddelta_bias,dstate_in,workspace z:workspace_bytes")
+LayerNormArgs, _ln_pack = _block(
+    "LayerNormArgs", "i:dtype,dim l:rows f:eps p:x l:x_stride p:weight,bias,y,mean,rstd,dy l:dy_stride "
+                     "p:dx,dweight,dbias,workspace z:workspace_bytes")
+ConvArgs, _conv_pack = _block(
+    "ConvArgs", "i:dtype,batch,length,dim,width,silu p:x l:x_batch,x_time p:weight,bias,lengths,state_in "
+                "l:state_in_batch p:state_out l:state_out_batch p:y,dy l:dy_batch,dy_time "
+                "p:dstate_out,dx,dstate_in,dweight,dbias,workspace z:workspace_bytes")
+ScanArgs, _scan_pack = _block(
+    "ScanArgs", "i:dtype,batch,length,dim,groups,nstate,softplus p:x,delta,z "
+                "l:x_batch,x_time,delta_batch,delta_time,z_batch,z_time p:B,C "
+                "l:B_batch,B_time,B_group,C_batch,C_time,C_group p:A,D,delta_bias,lengths,state_in "
+                "l:state_in_batch p:state_out l:state_out_batch p:saved,y,dy l:dy_batch,dy_time "
+                "p:dstate_out,dx,ddelta,dz,dB,dC,dA,dD,ddelta_bias,dstate_in,workspace z:workspace_bytes")
 
 _SERIES_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_F32 = torch.float32
 
 
-def _addr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -678,113 +691,126 @@ def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t (..., D) as rows (R, D) with one stride between rows."""
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t (..., D) with one stride between its rows, and that stride."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     t = _last_contiguous(t)
     try:
-        return t.view(-1, t.shape[-1])
+        return t, t.view(-1, t.shape[-1]).stride(0)
     except RuntimeError:
-        return t.contiguous().view(-1, t.shape[-1])
+        return t.contiguous(), t.shape[-1]
 
 
-def _params(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else _f32(t)
+def _param(t: torch.Tensor | None) -> torch.Tensor | None:
+    if t is None or (t.dtype is _F32 and t.is_contiguous()):
+        return t
+    return t.detach().to(_F32).contiguous()
 
 
-def _call(fn: str, what: str, args, device: torch.device) -> None:
+def _call(fn, what: str, block: bytes, device: torch.device) -> None:
     ev = _op_begin(device)
-    with _on(device):
-        rc = getattr(lib(), fn)(ctypes.byref(args), _stream(device))
-    _check(rc, what)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(block, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(block, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _check(rc, what)
     _op_end(what, device, ev)
 
 
-def _scratch(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def _new(like: torch.Tensor, shape=None, dtype=None, when: bool = True) -> torch.Tensor | None:
+    return torch.empty(like.shape if shape is None else shape, dtype=dtype or like.dtype, device=like.device) if when else None
 
 
 def layer_norm_forward(x, weight, bias, eps: float, stats: bool = True):
-    """(y, mean, rstd) of x (..., D); mean and rstd (rows,) float32, None without ``stats``."""
-    r = _rows(x)
-    rows, dim = r.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-    weight, bias = _params(weight), _params(bias)
-    a = LayerNormArgs(dtype=_SERIES_DTYPES[x.dtype], dim=dim, rows=rows, eps=eps, x=_addr(r), x_stride=r.stride(0),
-                      weight=_addr(weight), bias=_addr(bias), y=_addr(y), mean=_addr(mean), rstd=_addr(rstd))
-    _call("sdtw_layer_norm_forward", "layer_norm", a, x.device)
-    return y, mean, rstd
+    """(y, stats) of x (..., D); stats (2, rows) float32 holds each row's mean and 1 / deviation, or is None."""
+    r, stride = _rows(x)
+    dim = x.shape[-1]
+    rows = x.numel() // dim
+    y = _new(x)
+    weight, bias = _param(weight), _param(bias)
+    st, mean = None, 0
+    if stats:
+        st = _new(x, (2, rows), _F32)
+        mean = st.data_ptr()
+    _call(lib().sdtw_layer_norm_forward, "layer_norm",
+          _ln_pack(_SERIES_DTYPES[x.dtype], dim, rows, eps, r.data_ptr(), stride, _at(weight), _at(bias), y.data_ptr(), mean,
+                   mean + 4 * rows if stats else 0, 0, 0, 0, 0, 0, 0, 0), x.device)
+    return y, st
 
 
-def layer_norm_backward(x, weight, mean, rstd, dy, need_x=True, need_weight=True, need_bias=True):
+def layer_norm_backward(x, weight, stats, dy, need_x=True, need_weight=True, need_bias=True):
     """(dx, dweight, dbias); dweight and dbias (D,) float32, None where not needed."""
-    r, g = _rows(x), _rows(dy)
-    rows, dim = r.shape
-    weight = _params(weight)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    par = [torch.empty(dim, dtype=torch.float32, device=x.device) if need else None for need in (need_weight, need_bias)]
-    ws = _scratch(lib().sdtw_layer_norm_workspace_bytes(rows, dim), x.device) if need_weight or need_bias else None
-    a = LayerNormArgs(dtype=_SERIES_DTYPES[x.dtype], dim=dim, rows=rows, x=_addr(r), x_stride=r.stride(0),
-                      weight=_addr(weight), mean=_addr(mean), rstd=_addr(rstd), dy=_addr(g), dy_stride=g.stride(0),
-                      dx=_addr(dx), dweight=_addr(par[0]), dbias=_addr(par[1]), workspace=_addr(ws),
-                      workspace_bytes=0 if ws is None else ws.numel())
-    _call("sdtw_layer_norm_backward", "layer_norm gradient", a, x.device)
-    return dx, *par
-
-
-def _conv_args(x, weight, bias, silu, lengths, state_in, state_out):
-    batch, length, dim = x.shape
-    return ConvArgs(dtype=_SERIES_DTYPES[x.dtype], batch=batch, length=length, dim=dim, width=weight.shape[1],
-                    silu=int(silu), x=_addr(x), x_batch=x.stride(0), x_time=x.stride(1), weight=_addr(weight),
-                    bias=_addr(bias), lengths=_addr(lengths), state_in=_addr(state_in),
-                    state_in_batch=0 if state_in is None else state_in.stride(0), state_out=_addr(state_out),
-                    state_out_batch=0 if state_out is None else state_out.stride(0))
+    r, stride = _rows(x)
+    g, gstride = _rows(dy)
+    dim = x.shape[-1]
+    rows = x.numel() // dim
+    weight = _param(weight)
+    dx, dw, db = _new(x, when=need_x), _new(x, (dim,), _F32, need_weight), _new(x, (dim,), _F32, need_bias)
+    L = lib()
+    nbytes = L.sdtw_layer_norm_workspace_bytes(rows, dim) if need_weight or need_bias else 0
+    ws = _scratch(nbytes, x) if nbytes else None
+    mean = stats.data_ptr()
+    _call(L.sdtw_layer_norm_backward, "layer_norm gradient",
+          _ln_pack(_SERIES_DTYPES[x.dtype], dim, rows, 0.0, r.data_ptr(), stride, _at(weight), 0, 0, mean, mean + 4 * rows,
+                   g.data_ptr(), gstride, _at(dx), _at(dw), _at(db), _at(ws), nbytes), x.device)
+    return dx, dw, db
 
 
 def conv_forward(x, weight, bias, silu: bool, lengths, state_in, want_state: bool):
     """(y, state_out) of x (B, N, D), weight (D, W); state_out (B, W - 1, D) or None."""
-    x, weight, bias = _last_contiguous(x), _params(weight), _params(bias)
-    batch, _, dim = x.shape
+    x, weight, bias = _last_contiguous(x), _param(weight), _param(bias)
+    batch, length, dim = x.shape
+    width = weight.shape[1]
     state_in = None if state_in is None else state_in.contiguous()
-    state = torch.empty((batch, weight.shape[1] - 1, dim), dtype=x.dtype, device=x.device) if want_state else None
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _conv_args(x, weight, bias, silu, lengths, state_in, state)
-    a.y = _addr(y)
-    _call("sdtw_conv_forward", "causal_conv", a, x.device)
+    state = _new(x, (batch, width - 1, dim), when=want_state)
+    y = _new(x)
+    per = (width - 1) * dim
+    _call(lib().sdtw_conv_forward, "causal_conv",
+          _conv_pack(_SERIES_DTYPES[x.dtype], batch, length, dim, width, silu, x.data_ptr(), x.stride(0), x.stride(1),
+                     weight.data_ptr(), _at(bias), _at(lengths), _at(state_in), per, _at(state), per, y.data_ptr(),
+                     0, 0, 0, 0, 0, 0, 0, 0, 0, 0), x.device)
     return y, state
 
 
 def conv_backward(x, weight, bias, silu: bool, lengths, state_in, dy, dstate, need_x=True, need_weight=True,
                   need_bias=True, need_state=False):
     """(dx, dweight, dbias, dstate_in), None where not needed."""
-    x, weight, bias, dy = _last_contiguous(x), _params(weight), _params(bias), _last_contiguous(dy)
+    x, weight, bias, dy = _last_contiguous(x), _param(weight), _param(bias), _last_contiguous(dy)
     batch, length, dim = x.shape
     width = weight.shape[1]
     state_in = None if state_in is None else state_in.contiguous()
     dstate = None if dstate is None else dstate.contiguous()
-    dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty((dim, width), dtype=torch.float32, device=dev) if need_weight else None
-    db = torch.empty(dim, dtype=torch.float32, device=dev) if need_bias else None
-    ds = torch.empty((batch, width - 1, dim), dtype=x.dtype, device=dev) if need_state else None
-    ws = _scratch(lib().sdtw_conv_workspace_bytes(batch, length, dim, width), dev) if need_weight or need_bias else None
-    a = _conv_args(x, weight, bias, silu, lengths, state_in, None)
-    a.dy, a.dy_batch, a.dy_time = _addr(dy), dy.stride(0), dy.stride(1)
-    a.dstate_out, a.dx, a.dstate_in, a.dweight, a.dbias = _addr(dstate), _addr(dx), _addr(ds), _addr(dw), _addr(db)
-    a.workspace, a.workspace_bytes = _addr(ws), 0 if ws is None else ws.numel()
-    _call("sdtw_conv_backward", "causal_conv gradient", a, dev)
+    dx, dw, db = _new(x, when=need_x), _new(x, (dim, width), _F32, need_weight), _new(x, (dim,), _F32, need_bias)
+    ds = _new(x, (batch, width - 1, dim), when=need_state)
+    L = lib()
+    nbytes = L.sdtw_conv_workspace_bytes(batch, length, dim, width) if need_weight or need_bias else 0
+    ws = _scratch(nbytes, x) if nbytes else None
+    per = (width - 1) * dim
+    _call(L.sdtw_conv_backward, "causal_conv gradient",
+          _conv_pack(_SERIES_DTYPES[x.dtype], batch, length, dim, width, silu, x.data_ptr(), x.stride(0), x.stride(1),
+                     weight.data_ptr(), _at(bias), _at(lengths), _at(state_in), per, 0, 0, 0,
+                     dy.data_ptr(), dy.stride(0), dy.stride(1), _at(dstate), _at(dx), _at(ds), _at(dw), _at(db), _at(ws),
+                     nbytes), x.device)
     return dx, dw, db, ds
 
 
 def conv_step(x, weight, bias, silu: bool, state_in, state_out):
     """y (B, D) for x (B, D); state_out <- the window moved up by x (may be state_in)."""
-    x = _last_contiguous(x)
-    weight, bias = _params(weight), _params(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _conv_args(x.unsqueeze(1), weight, bias, silu, None, state_in, state_out)
-    a.y = _addr(y)
-    _call("sdtw_conv_step", "causal_conv step", a, x.device)
+    x, weight, bias = _last_contiguous(x), _param(weight), _param(bias)
+    y = _new(x)
+    batch, dim = x.shape
+    _call(lib().sdtw_conv_step, "causal_conv step",
+          _conv_pack(_SERIES_DTYPES[x.dtype], batch, 1, dim, weight.shape[1], silu, x.data_ptr(), x.stride(0), 0,
+                     weight.data_ptr(), _at(bias), 0, state_in.data_ptr(), state_in.stride(0), state_out.data_ptr(),
+                     state_out.stride(0), y.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), x.device)
     return y
 
 
@@ -792,70 +818,68 @@ def scan_saved_elems(batch: int, length: int, dim: int, nstate: int) -> int:
     return int(lib().sdtw_scan_saved_elems(batch, length, dim, nstate))
 
 
-def _scan_args(x, delta, A, B, C, D, z, bias, softplus, lengths, state_in, state_out):
-    batch, length, dim = x.shape
-    a = ScanArgs(dtype=_SERIES_DTYPES[x.dtype], batch=batch, length=length, dim=dim, groups=B.shape[2],
-                 nstate=A.shape[1], softplus=int(softplus), x=_addr(x), delta=_addr(delta), z=_addr(z),
-                 x_batch=x.stride(0), x_time=x.stride(1), delta_batch=delta.stride(0), delta_time=delta.stride(1),
-                 B=_addr(B), C=_addr(C), B_batch=B.stride(0), B_time=B.stride(1), B_group=B.stride(2),
-                 C_batch=C.stride(0), C_time=C.stride(1), C_group=C.stride(2), A=_addr(A), D=_addr(D),
-                 delta_bias=_addr(bias), lengths=_addr(lengths), state_in=_addr(state_in), state_out=_addr(state_out))
-    if z is not None:
-        a.z_batch, a.z_time = z.stride(0), z.stride(1)
-    if state_in is not None:
-        a.state_in_batch = state_in.stride(0)
-    if state_out is not None:
-        a.state_out_batch = state_out.stride(0)
-    return a
+def _scan_block(x, delta, A, B, C, D, z, bias, softplus, lengths, state_in, state_out, tail) -> bytes:
+    """x, delta, z (Bt, N, D) or, for a step, (Bt, D); B, C (Bt, N, G, S) or (Bt, G, S).  `tail`: from `saved` on."""
+    step = x.dim() == 2
+    dim, S = A.shape
+    # Strides of the batch, the time and the groups (no time for a step).
+    xb, db, zb = x.stride(0), delta.stride(0), 0 if z is None else z.stride(0)
+    xt, dt, zt = (0, 0, 0) if step else (x.stride(1), delta.stride(1), 0 if z is None else z.stride(1))
+    Bs, Cs = B.stride(), C.stride()
+    Bt, Ct = (0, 0) if step else (Bs[1], Cs[1])
+    return _scan_pack(_SERIES_DTYPES[x.dtype], x.shape[0], 1 if step else x.shape[1], dim, B.shape[-2], S, softplus,
+                      x.data_ptr(), delta.data_ptr(), _at(z), xb, xt, db, dt, zb, zt, B.data_ptr(), C.data_ptr(),
+                      Bs[0], Bt, Bs[-2], Cs[0], Ct, Cs[-2], A.data_ptr(), _at(D), _at(bias), _at(lengths), _at(state_in),
+                      0 if state_in is None else state_in.stride(0), _at(state_out),
+                      0 if state_out is None else state_out.stride(0), *tail)
 
 
 def _scan_inputs(x, delta, A, B, C, D, z, bias):
-    series = [None if t is None else _last_contiguous(t) for t in (x, delta, B, C, z)]
-    return (*series, *(_params(t) for t in (A, D, bias)))
+    return (_last_contiguous(x), _last_contiguous(delta), _param(A), _last_contiguous(B), _last_contiguous(C), _param(D),
+            None if z is None else _last_contiguous(z), _param(bias))
 
 
 def scan_forward(x, delta, A, B, C, D, z, bias, softplus: bool, lengths, state_in, want_state: bool, save: bool):
     """(y, state_out, saved) of x, delta, z (Bt, N, D), A (D, S), B, C (Bt, N, G, S)."""
-    x, delta, B, C, z, A, D, bias = _scan_inputs(x, delta, A, B, C, D, z, bias)
+    ins = _scan_inputs(x, delta, A, B, C, D, z, bias)
     batch, length, dim = x.shape
-    S = A.shape[1]
-    state_in = _params(state_in)
-    state = torch.empty((batch, dim, S), dtype=torch.float32, device=x.device) if want_state else None
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    saved = torch.empty(scan_saved_elems(batch, length, dim, S), dtype=torch.float32, device=x.device) if save else None
-    a = _scan_args(x, delta, A, B, C, D, z, bias, softplus, lengths, state_in, state)
-    a.y, a.saved = _addr(y), _addr(saved)
-    _call("sdtw_scan_forward", "selective_scan", a, x.device)
+    G, S = B.shape[2], A.shape[1]
+    L = lib()
+    state_in = _param(state_in)
+    state = _new(x, (batch, dim, S), _F32, want_state)
+    y = _new(x)
+    saved = _new(x, (L.sdtw_scan_saved_elems(batch, length, dim, S),), _F32) if save else None
+    nbytes = L.sdtw_scan_forward_workspace_bytes(batch, length, dim, G, S)
+    ws = _scratch(nbytes, x) if nbytes else None
+    tail = (_at(saved), y.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, _at(ws), nbytes)
+    _call(L.sdtw_scan_forward, "selective_scan", _scan_block(*ins, softplus, lengths, state_in, state, tail), x.device)
     return y, state, saved
 
 
 def scan_backward(x, delta, A, B, C, D, z, bias, softplus: bool, lengths, saved, dy, dstate, need):
     """Gradients of (x, delta, A, B, C, D, z, delta_bias, initial_state), None where ``need`` is false."""
-    x, delta, B, C, z, A, D, bias = _scan_inputs(x, delta, A, B, C, D, z, bias)
-    dy = _last_contiguous(dy)
-    dstate = _params(dstate)
+    ins = _scan_inputs(x, delta, A, B, C, D, z, bias)
+    dy, dstate = _last_contiguous(dy), _param(dstate)
     batch, length, dim = x.shape
-    S, G, dev, f32 = A.shape[1], B.shape[2], x.device, torch.float32
-    shapes = (((batch, length, dim), x.dtype), ((batch, length, dim), x.dtype), ((dim, S), f32),
-              ((batch, length, G, S), x.dtype), ((batch, length, G, S), x.dtype), ((dim,), f32),
-              ((batch, length, dim), x.dtype), ((dim,), f32), ((batch, dim, S), f32))
-    out = [torch.empty(s, dtype=dt, device=dev) if n else None for (s, dt), n in zip(shapes, need)]
-    ws = _scratch(lib().sdtw_scan_workspace_bytes(batch, length, dim, G, S), dev)
-    a = _scan_args(x, delta, A, B, C, D, z, bias, softplus, lengths, None, None)
-    a.saved, a.dy, a.dy_batch, a.dy_time, a.dstate_out = _addr(saved), _addr(dy), dy.stride(0), dy.stride(1), _addr(dstate)
-    for f, t in zip(("dx", "ddelta", "dA", "dB", "dC", "dD", "dz", "ddelta_bias", "dstate_in"), out):
-        setattr(a, f, _addr(t))
-    a.workspace, a.workspace_bytes = _addr(ws), ws.numel()
-    _call("sdtw_scan_backward", "selective_scan gradient", a, dev)
-    return out
+    G, S = B.shape[2], A.shape[1]
+    series, groups = x.shape, (batch, length, G, S)
+    dx, ddelta, dz = _new(x, series, None, need[0]), _new(x, series, None, need[1]), _new(x, series, None, need[6])
+    dB, dC = _new(x, groups, None, need[3]), _new(x, groups, None, need[4])
+    dA, dD, db = _new(x, (dim, S), _F32, need[2]), _new(x, (dim,), _F32, need[5]), _new(x, (dim,), _F32, need[7])
+    dh = _new(x, (batch, dim, S), _F32, need[8])
+    L = lib()
+    nbytes = L.sdtw_scan_workspace_bytes(batch, length, dim, G, S)
+    ws = _scratch(nbytes, x)
+    tail = (saved.data_ptr(), 0, dy.data_ptr(), dy.stride(0), dy.stride(1), _at(dstate), _at(dx), _at(ddelta), _at(dz), _at(dB),
+            _at(dC), _at(dA), _at(dD), _at(db), _at(dh), ws.data_ptr(), nbytes)
+    _call(L.sdtw_scan_backward, "selective_scan gradient", _scan_block(*ins, softplus, lengths, None, None, tail), x.device)
+    return [dx, ddelta, dA, dB, dC, dD, dz, db, dh]
 
 
 def scan_step(x, delta, A, B, C, D, z, bias, softplus: bool, state_in, state_out):
     """y (Bt, D) for x, delta, z (Bt, D), B, C (Bt, G, S); state_out <- the next state (may be state_in)."""
-    x, delta, B, C, z, A, D, bias = _scan_inputs(x, delta, A, B, C, D, z, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    one = [None if t is None else t.unsqueeze(1) for t in (x, delta, B, C, z)]
-    a = _scan_args(one[0], one[1], A, one[2], one[3], D, one[4], bias, softplus, None, state_in, state_out)
-    a.y = _addr(y)
-    _call("sdtw_scan_step", "selective_scan step", a, x.device)
+    ins = _scan_inputs(x, delta, A, B, C, D, z, bias)
+    y = _new(x)
+    tail = (0, y.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _call(lib().sdtw_scan_step, "selective_scan step", _scan_block(*ins, softplus, None, state_in, state_out, tail), x.device)
     return y

@@ -178,38 +178,35 @@ def _fake_grads(shapes, need, like: Tensor) -> list[Tensor]:
 
 
 @torch.library.custom_op("softdtw_cuda::layer_norm_forward", mutates_args=(), device_types="cuda")
-def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
-                       eps: float) -> tuple[Tensor, Tensor, Tensor]:
+def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> tuple[Tensor, Tensor]:
     return _native.layer_norm_forward(x, weight, bias, eps)
 
 
 @layer_norm_forward.register_fake
 def _(x, weight, bias, eps):
-    rows = x.numel() // x.shape[-1]
-    return (x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32))
+    return x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
 
 
 @torch.library.custom_op("softdtw_cuda::layer_norm_backward", mutates_args=(), device_types="cuda")
-def layer_norm_backward(x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, dy: Tensor,
-                        need: list[bool]) -> list[Tensor]:
-    return _pack(_native.layer_norm_backward(x, weight, mean, rstd, dy, *need), x)
+def layer_norm_backward(x: Tensor, weight: Optional[Tensor], stats: Tensor, dy: Tensor, need: list[bool]) -> list[Tensor]:
+    return _pack(_native.layer_norm_backward(x, weight, stats, dy, *need), x)
 
 
 @layer_norm_backward.register_fake
-def _(x, weight, mean, rstd, dy, need):
+def _(x, weight, stats, dy, need):
     D = (x.shape[-1],)
     return _fake_grads(((x.shape, x.dtype), (D, torch.float32), (D, torch.float32)), need, x)
 
 
 def _ln_setup(ctx, inputs, output):
     x, weight, bias, _ = inputs
-    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+    ctx.save_for_backward(x, weight, bias, output[1])
 
 
-def _ln_backward(ctx, dy, _dmean, _drstd):
-    x, weight, bias, mean, rstd = ctx.saved_tensors
+def _ln_backward(ctx, dy, _dstats):
+    x, weight, bias, stats = ctx.saved_tensors
     need = _need(ctx, 3)
-    return (*_unpack(layer_norm_backward(x, weight, mean, rstd, dy, need), (x, weight, bias), need), None)
+    return (*_unpack(layer_norm_backward(x, weight, stats, dy, need), (x, weight, bias), need), None)
 
 
 layer_norm_forward.register_autograd(_ln_backward, setup_context=_ln_setup)

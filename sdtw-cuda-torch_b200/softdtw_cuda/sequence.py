@@ -31,18 +31,19 @@ MAX_STATE = 64
 
 
 # ----------------------------------------------------------------------------- checks
-def _check_series(name: str, t: Tensor, like: Tensor | None = None, shape: tuple | None = None) -> None:
+def _check_series(name: str, t: Tensor, like: Tensor | None = None, shape=None) -> None:
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype not in _FLOAT_DTYPES:
-        raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
-    if like is not None:
-        if t.dtype != like.dtype:
-            raise TypeError(f"{name} must have x's dtype {like.dtype}, got {t.dtype}")
-        if t.device != like.device:
-            raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
+    if like is None:
+        if t.dtype not in _FLOAT_DTYPES:
+            raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
+        return
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must have x's dtype {like.dtype}, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}. Got {tuple(t.shape)}")
 
 
 def _check_param(name: str, t: Tensor | None, like: Tensor, shape: tuple) -> None:
@@ -54,7 +55,7 @@ def _check_param(name: str, t: Tensor | None, like: Tensor, shape: tuple) -> Non
         raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
     if t.device != like.device:
         raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
 
 
@@ -78,9 +79,9 @@ def _check_state(name: str, t: Tensor, like: Tensor, shape: tuple, dtype: torch.
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} must be on x's device {like.device}, got {t.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}. Got {tuple(t.shape)}")
-    if t.numel() and (not t[0].is_contiguous() or (shape[0] > 1 and t.stride(0) < t[0].numel())):
+    if not t.is_contiguous() and (not t[0].is_contiguous() or (shape[0] > 1 and t.stride(0) < t[0].numel())):
         raise ValueError(f"{name} must hold each batch entry contiguously, got strides {t.stride()}")
 
 
@@ -88,7 +89,7 @@ def _check_state_pair(state: Tensor, out: Tensor) -> None:
     """The new state may be written over the old one, but not over a part of it."""
     if out is state or not state.numel():
         return
-    B, inner, size = state.shape[0], state[0].numel(), state.element_size()
+    B, inner, size = state.shape[0], state.shape[1] * state.shape[2], state.element_size()
     s0, o0 = state.data_ptr(), out.data_ptr()
     ss, so = state.stride(0), out.stride(0)
     if s0 == o0 and (ss == so or B == 1):
@@ -102,7 +103,7 @@ def _check_state_pair(state: Tensor, out: Tensor) -> None:
 
 
 def _check_inference(what: str, *tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _tracked(*tensors):
         raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
 
 
@@ -117,7 +118,11 @@ def _on_kernels(x: Tensor) -> bool:
 
 
 def _tracked(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _wide(t: Tensor | None) -> Tensor | None:
@@ -126,22 +131,32 @@ def _wide(t: Tensor | None) -> Tensor | None:
 
 
 def _grad_as(g: Tensor | None, like: Tensor | None) -> Tensor | None:
-    return None if g is None else g.to(like.dtype)
+    return g if g is None or g.dtype is like.dtype else g.to(like.dtype)
+
+
+def _once(backward):
+    """once_differentiable, whose bookkeeping is skipped where no second derivative can follow."""
+    checked = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 # ----------------------------------------------------------------------------- layer norm
 class _LayerNorm(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _native.layer_norm_forward(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = _native.layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        dx, dw, db = _native.layer_norm_backward(x, weight, mean, rstd, dy, *ctx.needs_input_grad[:3])
+        x, weight, bias, stats = ctx.saved_tensors
+        dx, dw, db = _native.layer_norm_backward(x, weight, stats, dy, *ctx.needs_input_grad[:3])
         return dx, _grad_as(dw, weight), _grad_as(db, bias), None
 
 
@@ -190,7 +205,7 @@ class _CausalConv(Function):
         return y, state
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dstate):
         x, weight, bias, initial_state, lengths = ctx.saved_tensors
         if dy is None:
@@ -316,7 +331,7 @@ class _SelectiveScan(Function):
         return y, state
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dstate):
         x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, saved = ctx.saved_tensors
         if dy is None:
@@ -369,9 +384,9 @@ def _selective_scan_torch(x, delta, A, B, C, D, z, delta_bias, softplus, lengths
 
 def _check_scan(x, delta, A, B, C, D, z, delta_bias, seq: tuple):
     Dm = x.shape[-1]
-    _check_series("delta", delta, x, tuple(x.shape))
+    _check_series("delta", delta, x, x.shape)
     if z is not None:
-        _check_series("z", z, x, tuple(x.shape))
+        _check_series("z", z, x, x.shape)
     if not isinstance(A, Tensor) or A.dim() != 2 or A.shape[0] != Dm:
         raise ValueError(f"A must have shape ({Dm}, S). Got {tuple(getattr(A, 'shape', ()))}")
     S = A.shape[1]
@@ -379,13 +394,12 @@ def _check_scan(x, delta, A, B, C, D, z, delta_bias, seq: tuple):
         raise ValueError(f"A's state size must be between 1 and {MAX_STATE}, got {S}")
     _check_param("A", A, x, (Dm, S))
     _check_series("B", B, x)
-    _check_series("C", C, x)
     n = len(seq)
     if B.dim() not in (n + 1, n + 2) or tuple(B.shape[:n]) != seq or B.shape[-1] != S:
         raise ValueError(f"B must have shape {(*seq, S)} or {(*seq, 'G', S)}. Got {tuple(B.shape)}")
     if B.dim() == n + 2 and (B.shape[n] == 0 or Dm % B.shape[n]):
         raise ValueError(f"B's groups ({B.shape[n]}) must divide the features ({Dm})")
-    _check_series("C", C, x, tuple(B.shape))
+    _check_series("C", C, x, B.shape)
     _check_param("D", D, x, (Dm,))
     _check_param("delta_bias", delta_bias, x, (Dm,))
     if B.dim() == n + 1:

@@ -218,8 +218,8 @@ def test_fake_shapes():
     with FakeTensorMode():
         x = torch.empty(2, 40, 6, device="cuda", dtype=torch.bfloat16)
         f = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
-        y, mean, _ = torch.ops.softdtw_cuda.layer_norm_forward(x, f(6), None, 1e-5)
-        assert y.shape == x.shape and y.dtype == x.dtype and mean.shape == (80,)
+        y, stats = torch.ops.softdtw_cuda.layer_norm_forward(x, f(6), None, 1e-5)
+        assert y.shape == x.shape and y.dtype == x.dtype and stats.shape == (2, 80)
         y, st = torch.ops.softdtw_cuda.causal_conv_forward(x, f(6, 4), None, True, None, None, True)
         assert y.shape == x.shape and st.shape == (2, 3, 6)
         B = torch.empty(2, 40, 2, 5, device="cuda", dtype=torch.bfloat16)
