@@ -393,7 +393,7 @@ int sdtw_conv_step(const sdtw_conv_args *args, void *stream);
  * with the group g = d / (dim / groups).  h starts as state_in (NULL = zeros);
  * state_out, if given, gets h after each series' last valid step.  `saved`
  * (sdtw_scan_saved_elems floats; NULL when no backward follows) keeps the state
- * every 8 or 16 steps for the backward, which writes the gradients of every input
+ * every 16 steps for the backward, which writes the gradients of every input
  * (d* fields, each optional) from dy and dstate_out (optional).
  * sdtw_scan_step is the length-1 form for a running state:
  * state_in and state_out may be the same tensor, and lengths is not used. */

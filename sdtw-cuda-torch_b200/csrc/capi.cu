@@ -1472,7 +1472,7 @@ int sdtw_scan_backward(const sdtw_scan_args* a, void* stream) {
         if (int rc = check_workspace(a->workspace, a->workspace_bytes,
                                      scan_bwd_ws(a->batch, a->length, a->dim, a->groups, a->nstate)))
             return rc;
-        const bool split = scan_split(a->batch, a->length, a->dim, a->groups, a->nstate, true).nseg > 1;
+        const bool split = scan_split(a->batch, a->length, a->dim, a->groups, a->nstate).nseg > 1;
         return run_kernels("scan_bwd", split ? 3 : 2, stream, [&](cudaStream_t st) { return launch_scan_bwd(*a, st); });
     });
 }

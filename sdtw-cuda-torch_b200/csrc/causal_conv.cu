@@ -9,9 +9,11 @@
 // writes dx; W + 1 multiply-adds per element).  A thread owns VEC neighbouring
 // features and walks over a tile of time steps with the last W - 1 steps in
 // registers, so each element is read once and only the W - 1 steps before (and,
-// in the backward, behind) a tile twice.  The backward computes v again from x
-// instead of storing it, and keeps the thread's dw and dbias in registers; the
-// blocks' partial sums are added by a second kernel in a fixed order.
+// in the backward, behind) a tile twice.  The loads of the next steps are issued
+// before the present ones are worked on, and the multiply-adds are packed pairs
+// of features.  The backward computes v again from x instead of storing it, and
+// keeps the thread's dw and dbias in registers; the blocks' partial sums are
+// added by a second kernel in a fixed order.
 #include <algorithm>
 
 #include "seq_device.cuh"
@@ -21,12 +23,11 @@ namespace sdtw {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kU = 4;  // time steps whose loads are issued together
 
 struct ConvP {
     sdtw_conv_args a;
     int cx;      // threads over features (a power of two); kThreads / cx tiles per block
-    int tt;      // time steps per tile, a multiple of kU and >= 16
+    int tt;      // time steps per tile, a multiple of 16
     int nch;     // groups of VEC features
     int nchb;    // blocks over features
     int ntb;     // blocks over time
@@ -41,7 +42,9 @@ int conv_tile(int batch, int length, int nch) {
     while (tt > 16 && static_cast<long long>(batch) * ((length + tt - 1) / tt) * nch < 148ll * 1024) tt /= 2;
     return tt;
 }
-constexpr int kBwdVec = 4;  // 8 features' windows of x and gv, weights and dw would not fit in registers
+// Features per thread: 4 (8 or 16 bytes a load); 2 for a width that is not 2, 3
+// or 4, whose arrays of kConvMaxWidth taps would not fit in registers.
+constexpr int conv_vec(int width) { return width >= 2 && width <= 4 ? 4 : 2; }
 
 void conv_geometry(ConvP& p, int vec) {
     p.nch = (p.a.dim + vec - 1) / vec;
@@ -72,192 +75,210 @@ __device__ __forceinline__ void load_s(const ConvP& p, int b, int c, int n, int 
         v.zero();
 }
 
-template <typename T, int VEC, int WT>
-__device__ __forceinline__ void load_weights(const ConvP& p, int c, int n, int W, float (&w)[Width<WT>::kMax][VEC],
-                                             float (&bias)[VEC]) {
+// Taps from the newest step back: wr[m] = weight[W - 1 - m].  Features in pairs.
+template <int VEC, int WT>
+struct Taps {
+    static constexpr int KM = Width<WT>::kMax, VP = VEC / 2;
+    f2 wr[KM][VP], bias[VP];
+    __device__ __forceinline__ void load(const ConvP& p, int c, int n, int W) {
+        float v[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
+        for (int m = 0; m <= KM; ++m) {
 #pragma unroll
-        for (int k = 0; k < Width<WT>::kMax; ++k)
-            w[k][e] = (k < W && e < n) ? __ldg(p.a.weight + static_cast<long long>(c + e) * W + k) : 0.f;
-        bias[e] = (p.a.bias && e < n) ? __ldg(p.a.bias + c + e) : 0.f;
+            for (int e = 0; e < VEC; ++e) {
+                if (m < KM)
+                    v[e] = (m < W && e < n) ? __ldg(p.a.weight + static_cast<long long>(c + e) * W + (W - 1 - m)) : 0.f;
+                else
+                    v[e] = (p.a.bias && e < n) ? __ldg(p.a.bias + c + e) : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < VP; ++q) (m < KM ? wr[m < KM ? m : 0][q] : bias[q]) = pk(v[2 * q], v[2 * q + 1]);
+        }
     }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void to_pairs(const Vec<T, VEC>& r, f2 (&o)[VEC / 2]) {
+#pragma unroll
+    for (int q = 0; q < VEC / 2; ++q) o[q] = pk(r.get(2 * q), r.get(2 * q + 1));
 }
+
+// The block's place: a group of VEC features, a tile of time steps, a series.
+template <int VEC>
+struct ConvPlace {
+    int b, c, n, t0, t1, len, rest;
+    bool live, first;  // first tile of the series
+    __device__ __forceinline__ explicit ConvPlace(const ConvP& p) {
+        const int ci = (blockIdx.x % p.nchb) * p.cx + threadIdx.x % p.cx;
+        rest = blockIdx.x / p.nchb;
+        const int tile = (rest % p.ntb) * (kThreads / p.cx) + threadIdx.x / p.cx;
+        const long long t = static_cast<long long>(tile) * p.tt;
+        b = rest / p.ntb;
+        c = ci * VEC;
+        first = tile == 0;
+        live = ci < p.nch && t < p.a.length;
+        n = min(VEC, p.a.dim - c);
+        t0 = live ? static_cast<int>(t) : 0;
+        t1 = static_cast<int>(min(t + p.tt, static_cast<long long>(p.a.length)));
+        len = seq_len(p.a.lengths, b, p.a.length);
+    }
+};
 
 template <typename T, int VEC, int WT>
 __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
-    constexpr int KM = Width<WT>::kMax;
+    constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 8;
     const int W = Width<WT>::get(p.a.width);
-    const int ci = (blockIdx.x % p.nchb) * p.cx + threadIdx.x % p.cx;
-    const int rest = blockIdx.x / p.nchb;
-    const int tile = (rest % p.ntb) * (kThreads / p.cx) + threadIdx.x / p.cx;
-    const int b = rest / p.ntb;
-    const long long t0 = static_cast<long long>(tile) * p.tt;
-    const int c = ci * VEC;
-    if (ci >= p.nch || (t0 >= p.a.length)) return;
-    const int n = min(VEC, p.a.dim - c);
-    const int t1 = static_cast<int>(min(t0 + p.tt, static_cast<long long>(p.a.length)));
-    const int len = seq_len(p.a.lengths, b, p.a.length);
-    float w[KM][VEC], bias[VEC];
-    load_weights<T, VEC, WT>(p, c, n, W, w, bias);
-    float xs[KM - 1 + kU][VEC];  // xs[W - 1 + u]: step t + u; before it, its past
+    const ConvPlace<VEC> at(p);
+    if (!at.live) return;
+    const int c = at.c, n = at.n;
+    Taps<VEC, WT> k;
+    k.load(p, c, n, W);
+    f2 xs[KM - 1 + U][VP];  // xs[KM - 1 + u]: step t + u; before it, its past
 #pragma unroll
-    for (int k = 0; k < KM - 1; ++k)
-        if (k < W - 1) {
-            Vec<T, VEC> r;
-            load_s<T, VEC>(p, b, c, n, static_cast<int>(t0) + k, W, len, r);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) xs[k][e] = r.get(e);
-        }
-    const T* xp = static_cast<const T*>(p.a.x) + b * p.a.x_batch + c;
-    T* yp = static_cast<T*>(p.a.y) + static_cast<long long>(b) * p.a.length * p.a.dim + c;
-    for (int t = static_cast<int>(t0); t < t1; t += kU) {
-        Vec<T, VEC> raw[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            if (t + u < min(t1, len))
-                raw[u].load_n(xp + (t + u) * p.a.x_time, n, p.vec_x);
-            else
-                raw[u].zero();
-        }
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            float v[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float cur = raw[u].get(e);
-                v[e] = bias[e];
-                if constexpr (WT != 0) {
-                    xs[W - 1 + u][e] = cur;
-#pragma unroll
-                    for (int k = 0; k < KM; ++k) v[e] = fmaf(w[k][e], xs[k + u][e], v[e]);
-                } else {  // runtime width: xs holds the past, moved up at every step
-#pragma unroll
-                    for (int k = 0; k < KM; ++k)
-                        if (k < W) {
-                            const float s = k == W - 1 ? cur : xs[k][e];
-                            v[e] = fmaf(w[k][e], s, v[e]);
-                        }
-#pragma unroll
-                    for (int k = 0; k < KM - 1; ++k)
-                        if (k < W - 1) xs[k][e] = k == W - 2 ? cur : xs[k + 1][e];
-                }
-            }
-            if (t + u < t1) {
-                Vec<T, VEC> o;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float y = p.a.silu ? v[e] * sigmoidf(v[e]) : v[e];
-                    o.set(e, t + u < len ? y : 0.f);
-                }
-                o.store_n(yp + static_cast<long long>(t + u) * p.a.dim, n, p.vec_y);
-            }
-        }
-        if constexpr (WT != 0) {
-#pragma unroll
-            for (int k = 0; k < KM - 1; ++k)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) xs[k][e] = xs[k + kU][e];
-        }
+    for (int m = 1; m < KM; ++m) {
+        Vec<T, VEC> r;
+        r.zero();
+        if (m < W) load_s<T, VEC>(p, at.b, c, n, at.t0 + W - 1 - m, W, at.len, r);
+        to_pairs<T, VEC>(r, xs[KM - 1 - m]);
     }
-    if (p.a.state_out && tile == 0) {
-        for (int k = 0; k < W - 1; ++k) {
+    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + c;
+    T* yp = static_cast<T*>(p.a.y) + static_cast<long long>(at.b) * p.a.length * p.a.dim + c;
+    const int tl = min(at.t1, at.len);
+    Vec<T, VEC> next[U];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u].load_n(xp + (t + u) * p.a.x_time, t + u < tl ? n : 0, p.vec_x);
+    };
+    fetch(at.t0);
+    for (int t = at.t0; t < at.t1; t += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) to_pairs<T, VEC>(next[u], xs[KM - 1 + u]);
+        if (t + U < at.t1) fetch(t + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Vec<T, VEC> o;
+#pragma unroll
+            for (int q = 0; q < VP; ++q) {
+                f2 v = k.bias[q];
+#pragma unroll
+                for (int m = 0; m < KM; ++m)
+                    if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
+                float y[2];
+                upk(v, y[0], y[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (p.a.silu) y[e] *= sigmoidf(y[e]);
+                    o.set(2 * q + e, t + u < at.len ? y[e] : 0.f);
+                }
+            }
+            if (t + u < at.t1) o.store_n(yp + static_cast<long long>(t + u) * p.a.dim, n, p.vec_y);
+        }
+#pragma unroll
+        for (int m = 0; m < KM - 1; ++m)
+#pragma unroll
+            for (int q = 0; q < VP; ++q) xs[m][q] = xs[m + U][q];
+    }
+    if (p.a.state_out && at.first) {
+        for (int i = 0; i < W - 1; ++i) {
             Vec<T, VEC> r;
-            load_s<T, VEC>(p, b, c, n, len + k, W, len, r);
-            r.store_n(static_cast<T*>(p.a.state_out) + b * p.a.state_out_batch + static_cast<long long>(k) * p.a.dim + c, n, p.vec_so);
+            load_s<T, VEC>(p, at.b, c, n, at.len + i, W, at.len, r);
+            r.store_n(static_cast<T*>(p.a.state_out) + at.b * p.a.state_out_batch + static_cast<long long>(i) * p.a.dim + c, n, p.vec_so);
         }
     }
 }
 
 template <typename T, int VEC, int WT>
 __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
-    constexpr int KM = Width<WT>::kMax;
+    constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 4;
     const int W = Width<WT>::get(p.a.width);
-    const int tx = threadIdx.x % p.cx;
-    const int ci = (blockIdx.x % p.nchb) * p.cx + tx;
-    const int rest = blockIdx.x / p.nchb;
-    const int tile = (rest % p.ntb) * (kThreads / p.cx) + threadIdx.x / p.cx;
-    const int b = rest / p.ntb;
-    const long long t0l = static_cast<long long>(tile) * p.tt;
-    const int c = ci * VEC;
-    const bool live = ci < p.nch && t0l < p.a.length;
-    float dw[KM][VEC], db[VEC];
+    const ConvPlace<VEC> at(p);
+    const int rest = at.rest;
+    f2 dw[KM][VP], db[VP];  // dw[m]: of the tap m steps back
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        db[e] = 0.f;
+    for (int q = 0; q < VP; ++q) {
+        db[q] = pk(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < KM; ++k) dw[k][e] = 0.f;
+        for (int m = 0; m < KM; ++m) dw[m][q] = pk(0.f, 0.f);
     }
-    if (live) {
-        const int n = min(VEC, p.a.dim - c);
-        const int t0 = static_cast<int>(t0l);
-        const int t1 = min(t0 + p.tt, p.a.length);
-        const int len = seq_len(p.a.lengths, b, p.a.length);
-        float w[KM][VEC], bias[VEC];
-        load_weights<T, VEC, WT>(p, c, n, W, w, bias);
-        // The last W - 1 steps: of s oldest first, of gv newest first.
-        float xs[KM][VEC], gs[KM][VEC];
+    if (at.live) {
+        const int c = at.c, n = at.n, t0 = at.t0, t1 = at.t1, len = at.len;
+        Taps<VEC, WT> k;
+        k.load(p, c, n, W);
+        f2 xs[KM - 1 + U][VP], gs[KM - 1 + U][VP];  // s and gv, as in the forward
 #pragma unroll
-        for (int k = 0; k < KM; ++k) {
-            if (k < W - 1) {
-                Vec<T, VEC> r;
-                load_s<T, VEC>(p, b, c, n, t0 + k, W, len, r);
+        for (int m = 1; m < KM; ++m) {
+            Vec<T, VEC> r;
+            r.zero();
+            if (m < W) load_s<T, VEC>(p, at.b, c, n, t0 + W - 1 - m, W, len, r);
+            to_pairs<T, VEC>(r, xs[KM - 1 - m]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) xs[k][e] = r.get(e);
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gs[k][e] = 0.f;
+            for (int q = 0; q < VP; ++q) gs[KM - 1 - m][q] = pk(0.f, 0.f);
         }
-        const T* xp = static_cast<const T*>(p.a.x) + b * p.a.x_batch + c;
-        const T* gp = static_cast<const T*>(p.a.dy) + b * p.a.dy_batch + c;
-        T* dxp = static_cast<T*>(p.a.dx) + static_cast<long long>(b) * p.a.length * p.a.dim + c;
+        const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + c;
+        const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + c;
+        T* dxp = static_cast<T*>(p.a.dx) + static_cast<long long>(at.b) * p.a.length * p.a.dim + c;
         // Step j brings gv[j] and with it dL/ds[j], which is the gradient of
         // x[j - (W - 1)]; the W - 1 steps behind the tile complete its last ones.
-        const int j_end = t1 + W - 1;
-        for (int j0 = t0; j0 < j_end; j0 += kU) {
-            Vec<T, VEC> rx[kU], rg[kU];
+        const int j_end = t1 + W - 1, jl = min(j_end, len);
+        Vec<T, VEC> nx[U], ng[U];
+        auto fetch = [&](int j) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int nr = j0 + u < min(j_end, len) ? n : 0;
-                rx[u].load_n(xp + (j0 + u) * p.a.x_time, nr, p.vec_x);
-                rg[u].load_n(gp + (j0 + u) * p.a.dy_time, nr, p.vec_dy);
+            for (int u = 0; u < U; ++u) {
+                const int m = j + u < jl ? n : 0;
+                nx[u].load_n(xp + (j + u) * p.a.x_time, m, p.vec_x);
+                ng[u].load_n(gp + (j + u) * p.a.dy_time, m, p.vec_dy);
             }
+        };
+        fetch(t0);
+        for (int j0 = t0; j0 < j_end; j0 += U) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
+            for (int u = 0; u < U; ++u) {
+                to_pairs<T, VEC>(nx[u], xs[KM - 1 + u]);
+                to_pairs<T, VEC>(ng[u], gs[KM - 1 + u]);
+            }
+            if (j0 + U < j_end) fetch(j0 + U);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
                 const int j = j0 + u, t = j - (W - 1);
                 const bool own = j < t1;
                 float ds[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float cur = rx[u].get(e);
-                    float g = rg[u].get(e);
+                for (int q = 0; q < VP; ++q) {
+                    f2 g = gs[KM - 1 + u][q];
                     if (p.a.silu) {
-                        float v = bias[e];
+                        f2 v = k.bias[q];
 #pragma unroll
-                        for (int k = 0; k < KM; ++k)
-                            if (k < W) v = fmaf(w[k][e], k == W - 1 ? cur : xs[k][e], v);
-                        g *= dsilu(v);
+                        for (int m = 0; m < KM; ++m)
+                            if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
+                        float a, b;
+                        upk(v, a, b);
+                        g = mul2(g, pk(dsilu(a), dsilu(b)));
                     }
-                    if (j >= len) g = 0.f;
-                    if (own) db[e] += g;
-                    ds[e] = 0.f;
+                    if (j >= len) g = pk(0.f, 0.f);
+                    gs[KM - 1 + u][q] = g;
+                    if (own) {
+                        db[q] = add2(db[q], g);
 #pragma unroll
-                    for (int k = 0; k < KM; ++k)
-                        if (k < W) {
-                            if (own) dw[k][e] = fmaf(g, k == W - 1 ? cur : xs[k][e], dw[k][e]);
-                            ds[e] = fmaf(w[k][e], k == 0 ? g : gs[k > 0 ? k - 1 : 0][e], ds[e]);
-                        }
+                        for (int m = 0; m < KM; ++m)
+                            if (m < W) dw[m][q] = fma2(g, xs[KM - 1 + u - m][q], dw[m][q]);
+                    }
+                    // sum_k w[k] gv[j - k], w[k] = wr[W - 1 - k].
+                    f2 d = pk(0.f, 0.f);
+                    if constexpr (WT != 0) {
 #pragma unroll
-                    for (int k = 0; k < KM - 1; ++k)
-                        if (k < W - 1) xs[k][e] = k == W - 2 ? cur : xs[k + 1][e];
+                        for (int i = 0; i < KM; ++i) d = fma2(k.wr[KM - 1 - i][q], gs[KM - 1 + u - i][q], d);
+                    } else {
 #pragma unroll
-                    for (int k = KM - 1; k > 0; --k) gs[k][e] = gs[k - 1][e];
-                    gs[0][e] = g;
+                        for (int i = 0; i < KM; ++i)
+#pragma unroll
+                            for (int m = 0; m < KM; ++m)
+                                if (m + i == W - 1) d = fma2(k.wr[m][q], gs[KM - 1 + u - i][q], d);
+                    }
+                    upk(d, ds[2 * q], ds[2 * q + 1]);
                 }
                 if (p.a.dx && t >= t0 && t < t1) {
                     if (p.a.dstate_out && t < len && j >= len) {
                         Vec<T, VEC> r;
-                        r.load_n(static_cast<const T*>(p.a.dstate_out) + (static_cast<long long>(b) * (W - 1) + (j - len)) * p.a.dim + c, n,
+                        r.load_n(static_cast<const T*>(p.a.dstate_out) + (static_cast<long long>(at.b) * (W - 1) + (j - len)) * p.a.dim + c, n,
                                  p.vec_dso);
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) ds[e] += r.get(e);
@@ -268,6 +289,13 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
                     o.store_n(dxp + static_cast<long long>(t) * p.a.dim, n, p.vec_dx);
                 }
             }
+#pragma unroll
+            for (int m = 0; m < KM - 1; ++m)
+#pragma unroll
+                for (int q = 0; q < VP; ++q) {
+                    xs[m][q] = xs[m + U][q];
+                    gs[m][q] = gs[m + U][q];
+                }
         }
     }
     if (p.part == nullptr) return;
@@ -277,12 +305,12 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
     for (int k = 0; k <= W; ++k) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float v = db[e];
+        for (int q = 0; q < VP; ++q) {
+            f2 v = db[q];
 #pragma unroll
-            for (int q = 0; q < KM; ++q)
-                if (q == k && k < W) v = dw[q][e];
-            acc[threadIdx.x * VEC + e] = v;
+            for (int m = 0; m < KM; ++m)
+                if (m == W - 1 - k) v = dw[m][q];
+            upk(v, acc[threadIdx.x * VEC + 2 * q], acc[threadIdx.x * VEC + 2 * q + 1]);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < p.cx * VEC; i += kThreads) {
@@ -394,18 +422,18 @@ void conv_flags(ConvP& p) {
     p.vec_dso = d && vec_ok<T, VEC>(a.dstate_out, ds, 0);
 }
 
-template <typename T, int VEC, bool BWD>
+template <typename T, bool BWD>
 cudaError_t run_conv(const sdtw_conv_args& a, cudaStream_t st) {
     ConvP p{};
     p.a = a;
-    conv_geometry(p, VEC);
-    conv_flags<T, VEC>(p);
     if (BWD && (a.dweight || a.dbias)) p.part = static_cast<float*>(a.workspace);
-    const long long blocks = static_cast<long long>(p.nchb) * p.ntb * a.batch;
-    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    const unsigned g = static_cast<unsigned>(blocks);
+    conv_geometry(p, conv_vec(a.width));
+    if (static_cast<long long>(p.nchb) * p.ntb * a.batch > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     auto go = [&](auto width) {
-        constexpr int WT = decltype(width)::value;
+        constexpr int WT = decltype(width)::value, VEC = conv_vec(WT);
+        conv_geometry(p, VEC);
+        conv_flags<T, VEC>(p);
+        const unsigned g = static_cast<unsigned>(static_cast<long long>(p.nchb) * p.ntb * a.batch);
         if constexpr (BWD)
             conv_bwd_kernel<T, VEC, WT><<<g, kThreads, 0, st>>>(p);
         else
@@ -435,19 +463,19 @@ size_t conv_bwd_ws(int batch, int length, int dim, int width) {
     p.a.batch = batch;
     p.a.length = length;
     p.a.dim = dim;
-    conv_geometry(p, kBwdVec);
+    conv_geometry(p, conv_vec(width));
     return static_cast<size_t>(p.ntb) * batch * (width + 1) * static_cast<size_t>(dim) * sizeof(float);
 }
 
 cudaError_t launch_conv_fwd(const sdtw_conv_args& a, cudaStream_t st) {
-    if (a.dtype == SDTW_F32) return run_conv<float, 4, false>(a, st);
-    if (a.dtype == SDTW_F16) return run_conv<__half, 8, false>(a, st);
-    return run_conv<__nv_bfloat16, 8, false>(a, st);
+    if (a.dtype == SDTW_F32) return run_conv<float, false>(a, st);
+    if (a.dtype == SDTW_F16) return run_conv<__half, false>(a, st);
+    return run_conv<__nv_bfloat16, false>(a, st);
 }
 cudaError_t launch_conv_bwd(const sdtw_conv_args& a, cudaStream_t st) {
-    if (a.dtype == SDTW_F32) return run_conv<float, kBwdVec, true>(a, st);
-    if (a.dtype == SDTW_F16) return run_conv<__half, kBwdVec, true>(a, st);
-    return run_conv<__nv_bfloat16, kBwdVec, true>(a, st);
+    if (a.dtype == SDTW_F32) return run_conv<float, true>(a, st);
+    if (a.dtype == SDTW_F16) return run_conv<__half, true>(a, st);
+    return run_conv<__nv_bfloat16, true>(a, st);
 }
 cudaError_t launch_conv_step(const sdtw_conv_args& a, cudaStream_t st) {
     ConvP p{};

@@ -48,23 +48,77 @@ __device__ __forceinline__ float row_sum(float v, float (*buf)[TPR / 32], int& t
     return v;
 }
 
+// Weights and biases of the rows' features.  Rows of a warp or four read them
+// from shared memory at every row: in registers they would take the place of
+// further rows in flight.  Rows of 16 warps hold 16 features per thread and keep
+// them in registers.
+template <int VEC, int NV, int TPR>
+struct LnWeights {
+    static constexpr bool kShared = TPR <= 128;
+    static constexpr int kDim = kShared ? NV * VEC * TPR : 4;
+    float r[kShared ? 1 : NV * VEC];
+    const float* s;
+    __device__ __forceinline__ void load(const float* src, float none, int dim, float* buf, int tid) {
+        s = buf;
+        if constexpr (kShared) {
+            for (int c = threadIdx.x; c < kDim; c += blockDim.x) buf[c] = src && c < dim ? __ldg(src + c) : none;
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int c = (k * TPR + tid) * VEC + e;
+                    r[k * VEC + e] = src && c < dim ? __ldg(src + c) : none;
+                }
+        }
+    }
+    // The VEC values of piece k.
+    __device__ __forceinline__ void get(int k, int tid, float (&w)[VEC]) const {
+        if constexpr (!kShared) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) w[e] = r[k * VEC + e];
+        } else if constexpr (VEC % 4 == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(s + (k * TPR + tid) * VEC + e);
+                w[e] = v.x;
+                w[e + 1] = v.y;
+                w[e + 2] = v.z;
+                w[e + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) w[e] = s[(k * TPR + tid) * VEC + e];
+        }
+    }
+};
+
+__host__ __device__ constexpr int ln_threads(int tpr) { return tpr > 128 ? tpr : 128; }
+// Resident blocks to ask the compiler for: registers are the row's elements as
+// loaded (the next row's, and in the backward the present one's too) and the
+// float values in work (forward) or column sums (backward), and about 40 more.
+// Single 16-bit elements take a register each.
+__host__ __device__ constexpr int ln_blocks(int elems, int vec, int esize, int threads, bool bwd) {
+    const int raw = vec == 1 ? elems : elems * esize / 4;
+    const int regs = (bwd ? 2 * elems + 4 * raw : elems + raw) + 40;
+    const int n = 65536 / (threads * (regs > 250 ? 250 : regs));
+    return n < 1 ? 1 : (n > 8 ? 8 : n);
+}
+
 // Thread `tid` of a row holds the features (k TPR + tid) VEC .. + VEC, k < NV.
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_fwd_kernel(const LnP p) {
-    constexpr int RPB = TPR > 128 ? 1 : 128 / TPR;
+__global__ void __launch_bounds__(ln_threads(TPR), ln_blocks(VEC* NV, VEC, sizeof(T), ln_threads(TPR), false)) ln_fwd_kernel(const LnP p) {
+    constexpr int RPB = ln_threads(TPR) / TPR;
+    using Wt = LnWeights<VEC, NV, TPR>;
     __shared__ float buf[2][TPR / 32];
+    __shared__ __align__(16) float sw[Wt::kDim], sb[Wt::kDim];
     int turn = 0;
     const int tid = threadIdx.x % TPR;
     const float inv = 1.f / static_cast<float>(p.dim);
-    float w[NV * VEC], b[NV * VEC];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = (k * TPR + tid) * VEC + e;
-            w[k * VEC + e] = c < p.dim && p.w ? __ldg(p.w + c) : 1.f;
-            b[k * VEC + e] = c < p.dim && p.b ? __ldg(p.b + c) : 0.f;
-        }
+    Wt wt, bt;
+    wt.load(p.w, 1.f, p.dim, sw, tid);
+    bt.load(p.b, 0.f, p.dim, sb, tid);
+    __syncthreads();
     const long long step = static_cast<long long>(gridDim.x) * RPB;
     Vec<T, VEC> raw[NV];
     auto fetch = [&](long long r) {
@@ -72,10 +126,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_fwd_kernel(const LnP
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + tid) * VEC;
-            if (c < p.dim)
-                raw[k].load(xr + c);
-            else
-                raw[k].zero();
+            raw[k].load_n(xr + c, c < p.dim ? VEC : 0, true);
         }
     };
     long long r = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
@@ -104,10 +155,12 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_fwd_kernel(const LnP
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + tid) * VEC;
+            float w[VEC], b[VEC];
+            wt.get(k, tid, w);
+            bt.get(k, tid, b);
             Vec<T, VEC> o;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                o.set(e, fmaf(v[k * VEC + e] * rstd, w[k * VEC + e], b[k * VEC + e]));
+            for (int e = 0; e < VEC; ++e) o.set(e, fmaf(v[k * VEC + e] * rstd, w[e], b[e]));
             if (c < p.dim) o.store(yr + c);
         }
         if (tid == 0 && p.mean) {
@@ -117,63 +170,64 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_fwd_kernel(const LnP
     }
 }
 
+// The row's values are taken from the loaded pieces twice (for the sums and for
+// dx) rather than kept as floats.
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_bwd_kernel(const LnP p) {
-    constexpr int RPB = TPR > 128 ? 1 : 128 / TPR;
+__global__ void __launch_bounds__(ln_threads(TPR), ln_blocks(VEC* NV, VEC, sizeof(T), ln_threads(TPR), true)) ln_bwd_kernel(const LnP p) {
+    constexpr int RPB = ln_threads(TPR) / TPR;
+    using Wt = LnWeights<VEC, NV, TPR>;
     __shared__ float buf[2][TPR / 32];
+    __shared__ __align__(16) float sw[Wt::kDim];
     int turn = 0;
     const int tid = threadIdx.x % TPR;
     const float inv = 1.f / static_cast<float>(p.dim);
-    float w[NV * VEC], dw[NV * VEC], db[NV * VEC];
+    Wt wt;
+    wt.load(p.w, 1.f, p.dim, sw, tid);
+    __syncthreads();
+    float dw[NV * VEC], db[NV * VEC];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = (k * TPR + tid) * VEC + e;
-            w[k * VEC + e] = c < p.dim && p.w ? __ldg(p.w + c) : 1.f;
-            dw[k * VEC + e] = db[k * VEC + e] = 0.f;
-        }
+    for (int i = 0; i < NV * VEC; ++i) dw[i] = db[i] = 0.f;
     const long long step = static_cast<long long>(gridDim.x) * RPB;
-    Vec<T, VEC> rx[NV], rg[NV];
-    float mean = 0.f, rstd = 0.f;
+    Vec<T, VEC> nx[NV], ng[NV];
+    float nmean = 0.f, nrstd = 0.f;
     auto fetch = [&](long long r) {
         const T* xr = static_cast<const T*>(p.x) + r * p.xs;
         const T* gr = static_cast<const T*>(p.dy) + r * p.dys;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = (k * TPR + tid) * VEC;
-            if (c < p.dim) {
-                rx[k].load(xr + c);
-                rg[k].load(gr + c);
-            } else {
-                rx[k].zero();
-                rg[k].zero();
-            }
+            const int c = (k * TPR + tid) * VEC, n = c < p.dim ? VEC : 0;
+            nx[k].load_n(xr + c, n, true);
+            ng[k].load_n(gr + c, n, true);
         }
-        mean = __ldg(p.mean + r);
-        rstd = __ldg(p.rstd + r);
+        nmean = __ldg(p.mean + r);
+        nrstd = __ldg(p.rstd + r);
     };
     long long r = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
     if (r < p.rows) fetch(r);
     for (; r < p.rows; r += step) {
-        float xh[NV * VEC], g[NV * VEC];
-        float s1 = 0.f, s2 = 0.f;
-        const float rs = rstd;
+        Vec<T, VEC> rx[NV], rg[NV];
+        const float mean = nmean, rs = nrstd;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            rx[k] = nx[k];
+            rg[k] = ng[k];
+        }
+        if (r + step < p.rows) fetch(r + step);
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float w[VEC];
+            wt.get(k, tid, w);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int i = k * VEC + e;
-                const bool in = (k * TPR + tid) * VEC + e < p.dim;
-                xh[i] = in ? (rx[k].get(e) - mean) * rs : 0.f;
-                const float d = rg[k].get(e);
-                dw[i] = fmaf(d, xh[i], dw[i]);
-                db[i] += d;
-                g[i] = d * w[i];
-                s1 += g[i];
-                s2 = fmaf(g[i], xh[i], s2);
+                // Elements past the row read as x = dy = 0: only dy counts below.
+                const float xh = (rx[k].get(e) - mean) * rs, d = rg[k].get(e), g = d * w[e];
+                dw[k * VEC + e] = fmaf(d, xh, dw[k * VEC + e]);
+                db[k * VEC + e] += d;
+                s1 += g;
+                s2 = fmaf(g, xh, s2);
             }
-        if (r + step < p.rows) fetch(r + step);
+        }
         if (!p.want_dx) continue;
         s1 = row_sum<TPR>(s1, buf, turn) * inv;
         s2 = row_sum<TPR>(s2, buf, turn) * inv;
@@ -181,11 +235,13 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) ln_bwd_kernel(const LnP
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + tid) * VEC;
+            float w[VEC];
+            wt.get(k, tid, w);
             Vec<T, VEC> o;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int i = k * VEC + e;
-                o.set(e, rs * (g[i] - s1 - xh[i] * s2));
+                const float xh = (rx[k].get(e) - mean) * rs;
+                o.set(e, rs * (rg[k].get(e) * w[e] - s1 - xh * s2));
             }
             if (c < p.dim) o.store(dr + c);
         }
@@ -316,8 +372,8 @@ __global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int 
 // and longer rows (0) are not held at all.
 int threads_per_row(int dim) { return dim <= 32 * 32 ? 32 : (dim <= 128 * 32 ? 128 : (dim <= 512 * 16 ? 512 : 0)); }
 
-// Blocks of the backward, each of which leaves a partial row of column sums: as
-// many as are resident (16 warps per SM), but two rows per warp at least.
+// Blocks of the backward at most, each of which leaves a partial row of column
+// sums: as many as are resident (16 warps per SM), but two rows per warp at least.
 int bwd_blocks(long long rows, int dim) {
     const int tpr = threads_per_row(dim);
     if (tpr == 0) return static_cast<int>(std::min<long long>(rows, 64));
@@ -327,15 +383,17 @@ int bwd_blocks(long long rows, int dim) {
 }
 
 template <typename T, int VEC, int NV, int TPR>
-void run_ln(const LnP& p, bool bwd, int blocks, cudaStream_t st) {
-    constexpr int threads = TPR > 128 ? TPR : 128;
+void run_ln(const LnP& p, bool bwd, int& blocks, cudaStream_t st) {
+    constexpr int threads = ln_threads(TPR);
+    // No more blocks than are resident at once: each walks over its share of the rows.
+    blocks = std::min(blocks, 148 * ln_blocks(VEC * NV, VEC, sizeof(T), threads, bwd));
     if (bwd)
         ln_bwd_kernel<T, VEC, NV, TPR><<<blocks, threads, 0, st>>>(p);
     else
         ln_fwd_kernel<T, VEC, NV, TPR><<<blocks, threads, 0, st>>>(p);
 }
 template <typename T, int VEC, int NV>
-void run_ln_t(const LnP& p, int tpr, bool bwd, int blocks, cudaStream_t st) {
+void run_ln_t(const LnP& p, int tpr, bool bwd, int& blocks, cudaStream_t st) {
     if constexpr (VEC * NV <= 16)
         if (tpr == 512) return run_ln<T, VEC, NV, 512>(p, bwd, blocks, st);
     if (tpr == 128)
@@ -345,24 +403,24 @@ void run_ln_t(const LnP& p, int tpr, bool bwd, int blocks, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t run_ln_all(const LnP& p, bool bwd, cudaStream_t st) {
+cudaError_t run_ln_all(const LnP& p, bool bwd, int& blocks, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     const int tpr = threads_per_row(p.dim);
     if (tpr == 0) {
-        const int blocks = static_cast<int>(std::min<long long>(p.rows, 592));
+        blocks = static_cast<int>(std::min<long long>(p.rows, 592));
         if (!bwd) {
             ln_fwd_long_kernel<T><<<blocks, kLong, 0, st>>>(p);
         } else {
             if (p.want_dx) ln_bwd_long_kernel<T><<<blocks, kLong, 0, st>>>(p);
             if (p.want_part)
                 ln_cols_kernel<T><<<dim3((p.dim + 255) / 256, bwd_blocks(p.rows, p.dim)), 256, 0, st>>>(p);
+            blocks = bwd_blocks(p.rows, p.dim);
         }
         return cudaGetLastError();
     }
     const long long rpb = tpr == 32 ? 4 : 1;
     const int cap = tpr == 512 ? 296 : 1184;
-    const int blocks = bwd ? bwd_blocks(p.rows, p.dim)
-                           : static_cast<int>(std::min<long long>(cap, (p.rows + rpb - 1) / rpb));
+    blocks = bwd ? bwd_blocks(p.rows, p.dim) : static_cast<int>(std::min<long long>(cap, (p.rows + rpb - 1) / rpb));
     // 16-byte pieces when every row starts on one and ends with one; else single elements, lane by lane.
     const bool vec = p.dim % V == 0 && vec_ok<T, V>(p.x, p.xs, 0) &&
                      (bwd ? vec_ok<T, V>(p.dy, p.dys, 0) && vec_ok<T, V>(p.dx, 0, 0) : vec_ok<T, V>(p.y, 0, 0));
@@ -409,11 +467,12 @@ LnP ln_params(const sdtw_layer_norm_args& a) {
     return p;
 }
 
-cudaError_t run_ln_type(const sdtw_layer_norm_args& a, bool bwd, cudaStream_t st) {
+// `blocks`: how many ran, each of which left a partial row in the backward.
+cudaError_t run_ln_type(const sdtw_layer_norm_args& a, bool bwd, int& blocks, cudaStream_t st) {
     const LnP p = ln_params(a);
-    if (a.dtype == SDTW_F32) return run_ln_all<float>(p, bwd, st);
-    if (a.dtype == SDTW_F16) return run_ln_all<__half>(p, bwd, st);
-    return run_ln_all<__nv_bfloat16>(p, bwd, st);
+    if (a.dtype == SDTW_F32) return run_ln_all<float>(p, bwd, blocks, st);
+    if (a.dtype == SDTW_F16) return run_ln_all<__half>(p, bwd, blocks, st);
+    return run_ln_all<__nv_bfloat16>(p, bwd, blocks, st);
 }
 
 }  // namespace
@@ -422,13 +481,17 @@ size_t layer_norm_bwd_ws(long long rows, int dim) {
     return static_cast<size_t>(bwd_blocks(rows, dim)) * 2 * static_cast<size_t>(dim) * sizeof(float);
 }
 
-cudaError_t launch_layer_norm_fwd(const sdtw_layer_norm_args& a, cudaStream_t st) { return run_ln_type(a, false, st); }
+cudaError_t launch_layer_norm_fwd(const sdtw_layer_norm_args& a, cudaStream_t st) {
+    int blocks = 0;
+    return run_ln_type(a, false, blocks, st);
+}
 
 cudaError_t launch_layer_norm_bwd(const sdtw_layer_norm_args& a, cudaStream_t st) {
-    cudaError_t e = run_ln_type(a, true, st);
+    int blocks = 0;
+    cudaError_t e = run_ln_type(a, true, blocks, st);
     if (e != cudaSuccess || !(a.dweight || a.dbias)) return e;
     return launch_pdl(true, ln_reduce_kernel, dim3((2 * a.dim + 31) / 32), dim3(32, 32), 0, st,
-                      static_cast<const float*>(a.workspace), bwd_blocks(a.rows, a.dim), a.dim, a.dweight, a.dbias);
+                      static_cast<const float*>(a.workspace), blocks, a.dim, a.dweight, a.dbias);
 }
 
 }  // namespace sdtw

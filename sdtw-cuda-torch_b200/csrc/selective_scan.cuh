@@ -4,18 +4,22 @@
 //   dt = softplus(delta + bias),  u = dt x,  a[n] = exp(dt A[n])
 //   h[n] <- a[n] h[n] + u B[n],   y = sum_n C[n] h[n] + D x,   out = y z sigmoid(z)
 //
-// Tiling.  A thread owns 4 neighbouring states of 2 neighbouring features; NL
-// lanes side by side cover up to 4 NL states and the 32 / NL lane groups 64 / NL
-// features.  So B and C (one row of states per time step, shared by the
-// features) cost one 16-byte shared-memory load each per 8 state updates, dt and
-// u another, and the sums over the states are log2(NL) lane exchanges.  A warp
-// walks over the time steps; dt, u, B and C of TS steps at a time are staged in
-// shared memory, the elementwise functions computed once per element there.
+// Tiling.  A thread owns 4 neighbouring states of a feature; NL lanes side by
+// side cover up to 4 NL states and the 32 / NL lane groups as many neighbouring
+// features.  So a step costs a thread one 16-byte shared-memory load each of B
+// and C (rows of states, shared by the features) and 8 bytes of dt and u, and the
+// sums over the states are log2(NL) lane exchanges.  Two features per thread need
+// 15 % fewer instructions, but half as many warps can then work, and a warp issues
+// an instruction only every 5 to 6 cycles here (chains of exponentials, shared
+// loads and multiply-adds): measured on B200 at 32 x 512 x 512, 16 states,
+// bfloat16, 120 us forward and 285 us backward that way.
 //
-// Time.  When there are too few warps to fill the GPU, the time axis is cut into
-// segments: a first kernel runs each from h = 0 and keeps its end state E and
-// the sum of its dt (whose exponential with A is the product of the decays), and
-// the main kernel's warps chain the segments before their own,
+// Time.  A warp walks over the time steps; dt, u, B and C of 16 steps at a time
+// are staged in shared memory, the elementwise functions computed once per
+// element there.  When there are too few warps to fill the GPU, the time axis is
+// cut into segments: a first kernel runs each from h = 0 and keeps its end state E
+// and the sum of its dt (whose exponential with A is the product of the decays),
+// and the main kernel's warps chain the segments before their own,
 // h <- exp(A sum dt) h + E, before they start.  The exponentials are then
 // computed twice.
 #pragma once
@@ -27,19 +31,18 @@ namespace sdtw {
 
 constexpr int kScanWarps = 4;
 constexpr int kScanThreads = 32 * kScanWarps;
-constexpr int kCT = 2;     // features per thread
-constexpr int kRun = 8;    // time steps held in registers
+constexpr int kTS = kScanSave;  // staged time steps
+constexpr int kRun = 8;         // of them in registers at a time
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int NL>
 struct ScanTile {
-    static constexpr int CL = 32 / NL;               // lane groups over features
-    static constexpr int CH = CL * kCT;              // features per warp
-    static constexpr int NP = 4 * NL;                // states, padded
-    static constexpr int TS = scan_stage_steps(NL);  // staged time steps
-    static constexpr int LR = 32 / TS;               // staging lanes per time step
-    static constexpr int VX = CH / LR;               // features of a staging lane
-    static constexpr int VN = NP / LR;               // states of a staging lane
+    static constexpr int CH = 32 / NL;  // features per warp
+    static constexpr int NP = 4 * NL;   // states, padded
+    // Staging: two lanes per time step, each VX features and VN states.
+    static constexpr int LR = 32 / kTS;
+    static constexpr int VX = CH / LR;
+    static constexpr int VN = NP / LR;
 };
 
 struct ScanP {
@@ -48,6 +51,7 @@ struct ScanP {
     int tiles_g;   // warps' tiles per group
     int nchunk;    // stored states per series
     int nseg, seglen;
+    bool full;     // every tile has all its features and states, and every tensor its vector accesses
     bool vec_x, vec_delta, vec_z, vec_B, vec_C, vec_y, vec_dy, vec_dx, vec_ddelta, vec_dz;
     bool vec_n;    // the states of a thread are 16 bytes aligned
     float* seg_dt;    // (batch, nseg, dim) sums of dt
@@ -56,83 +60,107 @@ struct ScanP {
     float* part_par;  // backward: (batch, nseg, dim * nstate + 2 * dim) partial dA, dD, ddelta_bias
 };
 
-// A warp's place.  `tile` counts the warps over the features, all groups.
-template <int NL>
+// A warp's place: nc features of a group from c0 on, time steps t0 .. t1.
 struct ScanPlace {
-    int b, seg, g, c0, nc;
-    int t0, t1;  // the segment
-    __device__ __forceinline__ ScanPlace(const ScanP& p, int batch, int segment, int group, int tile_in_group) {
+    int b, seg, g, c0, nc, t0, t1;
+    __device__ __forceinline__ ScanPlace(const ScanP& p, int batch, int segment, int group, int tile_in_group, int features) {
         b = batch;
         seg = segment;
         g = group;
-        const int first = tile_in_group * ScanTile<NL>::CH;
+        const int first = tile_in_group * features;
         c0 = g * p.dg + first;
-        nc = max(0, min(ScanTile<NL>::CH, p.dg - first));
+        nc = max(0, min(features, p.dg - first));
         t0 = seg * p.seglen;
         t1 = min(t0 + p.seglen, p.a.length);
     }
-    __device__ static __forceinline__ ScanPlace of_warp(const ScanP& p, long long i) {
-        const int tiles = p.tiles_g * p.a.groups;
-        const int tile = static_cast<int>(i % tiles);
+    __device__ static __forceinline__ ScanPlace of_warp(const ScanP& p, long long i, int features) {
+        const int tiles = p.tiles_g * p.a.groups, tile = static_cast<int>(i % tiles);
         const long long bs = i / tiles;
-        return ScanPlace(p, static_cast<int>(bs / p.nseg), static_cast<int>(bs % p.nseg), tile / p.tiles_g, tile % p.tiles_g);
+        return ScanPlace(p, static_cast<int>(bs / p.nseg), static_cast<int>(bs % p.nseg), tile / p.tiles_g, tile % p.tiles_g, features);
     }
 };
 
-// A thread's 4 states of 2 features, as pairs [feature][pair].  Lanes with an
-// odd state group hold their two features swapped (see pair_exchange).
+// A thread's 4 states, in pairs.
 struct St {
-    f2 v[kCT][2];
+    f2 v[2];
 };
-__device__ __forceinline__ void st_set(St& s, float x) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) s.v[i][0] = s.v[i][1] = pk(x, x);
-}
-// States n0 .. n0 + 4 of features f + (0 ^ swap) and f + (1 ^ swap) of a
-// (features, S) table; those that do not exist read as 0 and are not written.
-__device__ __forceinline__ void st_load(St& s, const float* tab, int f, int swap, int nf, int S, int n0, bool vec) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) {
-        const int c = f + (i ^ swap);
-        Vec<float, 4> r;
-        const int n = c < nf ? min(max(S - n0, 0), 4) : 0;
-        r.load_n(tab + static_cast<long long>(c) * S + n0, n, vec);
-        s.v[i][0] = pk(r.get(0), r.get(1));
-        s.v[i][1] = pk(r.get(2), r.get(3));
-    }
-}
-__device__ __forceinline__ void st_store(const St& s, float* tab, int f, int swap, int nf, int S, int n0, bool vec) {
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) {
-        const int c = f + (i ^ swap);
-        Vec<float, 4> r;
-        float v[4];
-        upk(s.v[i][0], v[0], v[1]);
-        upk(s.v[i][1], v[2], v[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.set(j, v[j]);
-        const int n = c < nf ? min(max(S - n0, 0), 4) : 0;
-        r.store_n(tab + static_cast<long long>(c) * S + n0, n, vec);
-    }
-}
-// h <- exp(A sum dt) h + E over one segment.
-__device__ __forceinline__ void st_chain(St& h, const ScanP& p, const St& A2, int b, int seg, int f, int swap, int nf, int n0) {
-    const long long row = static_cast<long long>(b) * p.nseg + seg;
-    St E;
-    st_load(E, p.seg_E + row * p.a.dim * p.a.nstate, f, swap, nf, p.a.nstate, n0, p.vec_n);
-#pragma unroll
-    for (int i = 0; i < kCT; ++i) {
-        const int c = f + (i ^ swap);
-        const float d = c < nf ? __ldg(p.seg_dt + row * p.a.dim + c) : 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) h.v[i][j] = fma2(ex22(mul2(pk(d, d), A2.v[i][j])), h.v[i][j], E.v[i][j]);
-    }
-}
+__device__ __forceinline__ void st_set(St& s, float x) { s.v[0] = s.v[1] = pk(x, x); }
 __device__ __forceinline__ void st_scale(St& s, float k) {
+    s.v[0] = mul2(s.v[0], pk(k, k));
+    s.v[1] = mul2(s.v[1], pk(k, k));
+}
+// States n0 .. n0 + 4 of row `row` of a (rows, S) table; n of them exist.
+__device__ __forceinline__ St st_load(const float* tab, long long row, int S, int n0, int n, bool vec) {
+    Vec<float, 4> r;
+    r.load_n(tab + row * S + n0, n, vec);
+    return St{{pk(r.get(0), r.get(1)), pk(r.get(2), r.get(3))}};
+}
+__device__ __forceinline__ void st_store(const St& s, float* tab, long long row, int S, int n0, int n, bool vec) {
+    Vec<float, 4> r;
+    float v[4];
+    upk(s.v[0], v[0], v[1]);
+    upk(s.v[1], v[2], v[3]);
 #pragma unroll
-    for (int i = 0; i < kCT; ++i)
+    for (int j = 0; j < 4; ++j) r.set(j, v[j]);
+    r.store_n(tab + row * S + n0, n, vec);
+}
+__device__ __forceinline__ f2 half_of(ulonglong2 v, int j) { return f2{j ? v.y : v.x}; }
+// h <- exp(A sum dt) h + E over one segment.
+__device__ __forceinline__ void st_chain(St& h, const ScanP& p, const St& A2, int b, int seg, int f, int n0, int n) {
+    const long long row = (static_cast<long long>(b) * p.nseg + seg) * p.a.dim + f;
+    const St E = st_load(p.seg_E, row, p.a.nstate, n0, n, p.vec_n);
+    const float d = n > 0 ? __ldg(p.seg_dt + row) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s.v[i][j] = mul2(s.v[i][j], pk(k, k));
+    for (int j = 0; j < 2; ++j) h.v[j] = fma2(ex22(mul2(pk(d, d), A2.v[j])), h.v[j], E.v[j]);
+}
+
+// Loads of a staging lane: n elements (0 or all of them when FULL).
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void stage_load(Vec<T, V>& r, const T* q, int n, bool vec) {
+    if constexpr (FULL) {
+        r.zero();
+        if (n > 0) r.load(q);
+    } else {
+        r.load_n(q, n, vec);
+    }
+}
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void stage_store(const Vec<T, V>& r, T* q, int n, bool vec) {
+    if constexpr (FULL) {
+        if (n > 0) r.store(q);
+    } else {
+        r.store_n(q, n, vec);
+    }
+}
+// V floats to shared memory in pieces of at most 16 bytes.
+template <int V>
+__device__ __forceinline__ void put_floats(float* d, const float (&v)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(d + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) *reinterpret_cast<float2*>(d + e) = make_float2(v[e], v[e + 1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = v[e];
+    }
+}
+template <int V>
+__device__ __forceinline__ void get_floats(float (&v)[V], const float* s) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(s + e);
+            v[e] = q.x;
+            v[e + 1] = q.y;
+            v[e + 2] = q.z;
+            v[e + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = s[e];
+    }
 }
 
 template <typename T, int NL>
@@ -141,7 +169,7 @@ inline void scan_params(ScanP& p, const sdtw_scan_args& a) {
     p.a = a;
     p.dg = a.dim / a.groups;
     p.tiles_g = (p.dg + K::CH - 1) / K::CH;
-    p.nchunk = (a.length + K::TS - 1) / K::TS;
+    p.nchunk = (a.length + kScanSave - 1) / kScanSave;
     const bool d = p.dg % K::VX == 0;
     const long long ds = a.dim;
     p.vec_x = d && vec_ok<T, K::VX>(a.x, a.x_batch, a.x_time);
@@ -158,6 +186,8 @@ inline void scan_params(ScanP& p, const sdtw_scan_args& a) {
     p.vec_n = a.nstate % 4 == 0 && vec_ok<float, 4>(a.A, 0, 0) && vec_ok<float, 4>(a.state_in, a.state_in_batch, 0) &&
               vec_ok<float, 4>(a.state_out, a.state_out_batch, 0) && vec_ok<float, 4>(a.saved, 0, 0) &&
               vec_ok<float, 4>(a.dstate_in, 0, 0) && vec_ok<float, 4>(a.dstate_out, 0, 0);
+    p.full = p.dg % K::CH == 0 && a.nstate == K::NP && p.vec_x && p.vec_delta && p.vec_z && p.vec_y && p.vec_dy && p.vec_dx &&
+             p.vec_ddelta && p.vec_dz && p.vec_B && p.vec_C && p.vec_n;
 }
 
 // The segments' tables at the start of a workspace, and their floats.

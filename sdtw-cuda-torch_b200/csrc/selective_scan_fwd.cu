@@ -10,162 +10,166 @@ namespace {
 
 // One warp per (series, segment, tile of features); the warps of a block do not
 // wait for one another.
-template <typename T, int NL>
-__global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const ScanP p, long long warps) {
+template <typename T, int NL, bool FULL>
+__global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 3) scan_fwd_kernel(const ScanP p, long long warps) {
     using K = ScanTile<NL>;
-    // (dt, u) of two features, and once more with the two swapped; later y in the first.
-    __shared__ float4 sU[kScanWarps][2][K::TS][K::CH / 2];
-    __shared__ __align__(16) float sB[kScanWarps][K::TS][K::NP], sC[kScanWarps][K::TS][K::NP];
+    __shared__ __align__(16) float2 sU[kScanWarps][kTS][K::CH];  // (dt, u)
+    __shared__ __align__(16) float sB[kScanWarps][kTS][K::NP], sC[kScanWarps][kTS][K::NP], sY[kScanWarps][kTS][K::CH];
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long wi = static_cast<long long>(blockIdx.x) * kScanWarps + w;
     if (wi >= warps) return;
-    const ScanPlace<NL> at = ScanPlace<NL>::of_warp(p, wi);
-    const int nl = lane % NL, cl = lane / NL, swap = nl & 1, n0 = nl * 4;
+    const ScanPlace at = ScanPlace::of_warp(p, wi, K::CH);
+    const int nl = lane % NL, cl = lane / NL, n0 = nl * 4;
     const int S = p.a.nstate, L = p.a.length, dim = p.a.dim;
     const int len = seq_len(p.a.lengths, at.b, L);
-    const int f0 = at.c0 + cl * kCT, fend = at.c0 + at.nc;
+    const int f = at.c0 + cl, ns = FULL ? 4 : (cl < at.nc ? min(max(S - n0, 0), 4) : 0);
     const int row = lane / K::LR, col = lane % K::LR * K::VX, bcol = lane % K::LR * K::VN;
-    const int nx = min(max(at.nc - col, 0), K::VX), nb = min(max(S - bcol, 0), K::VN);
+    const int nx = FULL ? K::VX : min(max(at.nc - col, 0), K::VX), nb = FULL ? K::VN : min(max(S - bcol, 0), K::VN);
+    const bool vn = FULL || p.vec_n;
 
-    St A2, h;
-    st_load(A2, p.a.A, f0, swap, fend, S, n0, p.vec_n);
+    St A2 = st_load(p.a.A, f, S, n0, ns, vn), h;
     st_scale(A2, kL2e);
     st_set(h, 0.f);
-    if (p.a.state_in) st_load(h, p.a.state_in + at.b * p.a.state_in_batch, f0, swap, fend, S, n0, p.vec_n);
+    if (p.a.state_in) h = st_load(p.a.state_in + at.b * p.a.state_in_batch, f, S, n0, ns, vn);
     if (p.nseg > 1) {
         pdl_wait();
-        for (int q = 0; q < at.seg; ++q) st_chain(h, p, A2, at.b, q, f0, swap, fend, n0);
+#pragma unroll 4
+        for (int q = 0; q < at.seg; ++q) st_chain(h, p, A2, at.b, q, f, n0, ns);
     }
-    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + at.c0 + col;
-    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0 + col;
-    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0 + col;
-    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + at.g * p.a.B_group + bcol;
-    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + at.g * p.a.C_group + bcol;
-    T* yp = static_cast<T*>(p.a.y) + static_cast<long long>(at.b) * L * dim + at.c0 + col;
-    const float* bias = p.a.delta_bias ? p.a.delta_bias + at.c0 + col : nullptr;
-    const float* skip = p.a.D ? p.a.D + at.c0 + col : nullptr;
+    float bias[K::VX], skip[K::VX];
+#pragma unroll
+    for (int e = 0; e < K::VX; ++e) {
+        bias[e] = p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f;
+        skip[e] = p.a.D && e < nx ? __ldg(p.a.D + at.c0 + col + e) : 0.f;
+    }
+    const int r0 = at.t0 + row;  // the first step that this lane stages
+    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + r0 * p.a.x_time + at.c0 + col;
+    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + r0 * p.a.delta_time + at.c0 + col;
+    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + r0 * p.a.z_time + at.c0 + col;
+    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + r0 * p.a.B_time + at.g * p.a.B_group + bcol;
+    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + r0 * p.a.C_time + at.g * p.a.C_group + bcol;
+    T* yp = static_cast<T*>(p.a.y) + (static_cast<long long>(at.b) * L + r0) * dim + at.c0 + col;
+    float* sp = p.a.saved ? p.a.saved + (static_cast<long long>(at.b) * p.nchunk + at.t0 / kScanSave) * dim * S : nullptr;
 
     Vec<T, K::VX> rx, rd;
     Vec<T, K::VN> rB, rC;
     auto fetch = [&](int t) {
         const bool in = t < len;
-        rx.load_n(xp + t * p.a.x_time, in ? nx : 0, p.vec_x);
-        rd.load_n(dp + t * p.a.delta_time, in ? nx : 0, p.vec_delta);
-        rB.load_n(Bp + t * p.a.B_time, in ? nb : 0, p.vec_B);
-        rC.load_n(Cp + t * p.a.C_time, in ? nb : 0, p.vec_C);
+        stage_load<FULL>(rx, xp, in ? nx : 0, p.vec_x);
+        stage_load<FULL>(rd, dp, in ? nx : 0, p.vec_delta);
+        stage_load<FULL>(rB, Bp, in ? nb : 0, p.vec_B);
+        stage_load<FULL>(rC, Cp, in ? nb : 0, p.vec_C);
+        xp += kTS * p.a.x_time;
+        dp += kTS * p.a.delta_time;
+        Bp += kTS * p.a.B_time;
+        Cp += kTS * p.a.C_time;
     };
     const int tend = min(at.t1, len);
-    if (at.t0 < tend) fetch(at.t0 + row);
+    if (at.t0 < tend) fetch(r0);
     int tc = at.t0;
-    for (; tc < tend; tc += K::TS) {
-        const int t = tc + row;  // the step that this lane stages
+    for (; tc < tend; tc += kTS) {
+        const int t = tc + row;
+        const bool in = t < len;
         const Vec<T, K::VX> xk = rx;
         Vec<T, K::VX> rz;
-        if (p.a.z) rz.load_n(zp + t * p.a.z_time, t < len ? nx : 0, p.vec_z);
+        if (p.a.z) {
+            stage_load<FULL>(rz, zp, in ? nx : 0, p.vec_z);
+            zp += kTS * p.a.z_time;
+        }
         __syncwarp();
+        {
+            float v[2 * K::VX], b[K::VN], c[K::VN];
 #pragma unroll
-        for (int e = 0; e < K::VX; e += 2) {
-            float dt[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                dt[k] = rd.get(e + k) + (bias && e + k < nx ? __ldg(bias + e + k) : 0.f);
-                if (p.a.softplus) dt[k] = softplusf(dt[k]);
-                if (t >= len) dt[k] = 0.f;  // the state stays as it is
+            for (int e = 0; e < K::VX; ++e) {
+                float dt = rd.get(e) + bias[e];
+                if (p.a.softplus) dt = softplusf(dt);
+                dt = in ? dt : 0.f;  // the state stays as it is
+                v[2 * e] = dt;
+                v[2 * e + 1] = dt * rx.get(e);
             }
-            const float u0 = dt[0] * rx.get(e), u1 = dt[1] * rx.get(e + 1);
-            sU[w][0][row][(col + e) / 2] = make_float4(dt[0], u0, dt[1], u1);
-            sU[w][1][row][(col + e) / 2] = make_float4(dt[1], u1, dt[0], u0);
-        }
+            put_floats(reinterpret_cast<float*>(&sU[w][row][col]), v);
 #pragma unroll
-        for (int e = 0; e < K::VN; ++e) {
-            sB[w][row][bcol + e] = rB.get(e);
-            sC[w][row][bcol + e] = rC.get(e);
+            for (int e = 0; e < K::VN; ++e) {
+                b[e] = rB.get(e);
+                c[e] = rC.get(e);
+            }
+            put_floats(&sB[w][row][bcol], b);
+            put_floats(&sC[w][row][bcol], c);
         }
-        if (tc + K::TS < tend) fetch(t + K::TS);
+        if (tc + kTS < tend) fetch(t + kTS);
         __syncwarp();
-        if (p.a.saved)
-            st_store(h, p.a.saved + (static_cast<long long>(at.b) * p.nchunk + tc / K::TS) * dim * S, f0, swap, fend, S, n0, p.vec_n);
+        if (sp) {
+            st_store(h, sp, f, S, n0, ns, vn);
+            sp += static_cast<long long>(dim) * S;
+        }
 #pragma unroll 1
-        for (int sb = 0; sb < K::TS; sb += kRun) {
-            float v[kRun * kCT];
+        for (int sb = 0; sb < kTS; sb += kRun) {
+            float v[kRun];
 #pragma unroll
             for (int s = 0; s < kRun; ++s) {
-                const float4 du = sU[w][swap][sb + s][cl];
+                const float2 du = sU[w][sb + s][cl];
                 const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[w][sb + s][n0]);
                 const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sC[w][sb + s][n0]);
 #pragma unroll
-                for (int i = 0; i < kCT; ++i) {
-                    const float dt = i ? du.z : du.x, u = i ? du.w : du.y;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const f2 a = ex22(mul2(pk(dt, dt), A2.v[i][j]));
-                        h.v[i][j] = fma2(a, h.v[i][j], mul2(pk(u, u), f2{j ? bv.y : bv.x}));
-                    }
-                    v[s * kCT + i] = sum2(fma2(f2{cv.y}, h.v[i][1], mul2(f2{cv.x}, h.v[i][0])));
+                for (int j = 0; j < 2; ++j) {
+                    const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j]));
+                    h.v[j] = fma2(a, h.v[j], mul2(pk(du.y, du.y), half_of(bv, j)));
                 }
+                v[s] = sum2(fma2(half_of(cv, 1), h.v[1], mul2(half_of(cv, 0), h.v[0])));
             }
-            if constexpr (NL == 1) {
-                __syncwarp();
-#pragma unroll
-                for (int s = 0; s < kRun; ++s)
-                    *reinterpret_cast<float2*>(reinterpret_cast<float*>(sU[w][0][sb + s]) + cl * kCT) = make_float2(v[2 * s], v[2 * s + 1]);
-            } else {
-                float y[kRun];  // per step, of the lane's first feature
-                pair_exchange(v, y, 1);
-                using Sum = LaneSum<kRun, 2, NL / 2>;
-                Sum::run(y, lane);
-                __syncwarp();
+            using Sum = LaneSum<kRun, 1, NL>;
+            Sum::run(v, lane);
+            if (Sum::owner(lane)) {
                 const int slot = Sum::slot(lane);
 #pragma unroll
-                for (int k = 0; k < Sum::kept; ++k)
-                    reinterpret_cast<float*>(sU[w][0][sb + slot + k])[cl * kCT + swap] = y[k];
+                for (int k = 0; k < Sum::kept; ++k) sY[w][sb + slot + k][cl] = v[k];
             }
         }
         __syncwarp();
+        float y[K::VX];
+        get_floats(y, &sY[w][row][col]);
         Vec<T, K::VX> o;
-        const float* sY = reinterpret_cast<const float*>(sU[w][0][row]) + col;
 #pragma unroll
         for (int e = 0; e < K::VX; ++e) {
-            float y = fmaf(skip && e < nx ? __ldg(skip + e) : 0.f, xk.get(e), sY[e]);
+            y[e] = fmaf(skip[e], xk.get(e), y[e]);
             if (p.a.z) {
                 const float z = rz.get(e);
-                y *= z * sigmoidf(z);
+                y[e] *= z * sigmoidf(z);
             }
-            o.set(e, t < len ? y : 0.f);
+            o.set(e, in ? y[e] : 0.f);
         }
-        o.store_n(yp + static_cast<long long>(t) * dim, t < at.t1 ? nx : 0, p.vec_y);
+        stage_store<FULL>(o, yp, t < at.t1 ? nx : 0, p.vec_y);
+        yp += static_cast<long long>(kTS) * dim;
     }
-    for (int t = tc + row; t < at.t1; t += K::TS) {
+    for (int t = tc + row; t < at.t1; t += kTS) {
         Vec<T, K::VX> o;
         o.zero();
-        o.store_n(yp + static_cast<long long>(t) * dim, nx, p.vec_y);
+        stage_store<FULL>(o, yp, nx, p.vec_y);
+        yp += static_cast<long long>(kTS) * dim;
     }
-    if (p.a.state_out && at.seg == p.nseg - 1)
-        st_store(h, p.a.state_out + at.b * p.a.state_out_batch, f0, swap, fend, S, n0, p.vec_n);
+    if (p.a.state_out && at.seg == p.nseg - 1) st_store(h, p.a.state_out + at.b * p.a.state_out_batch, f, S, n0, ns, vn);
 }
 
 // End state and sum of dt of a segment run from 0: see launch_scan_segments.
 template <typename T, int NL, bool REV>
 __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP p, long long warps) {
     using K = ScanTile<NL>;
-    __shared__ float4 sU[kScanWarps][2][K::TS][K::CH / 2];
-    __shared__ __align__(16) float sB[kScanWarps][K::TS][K::NP];
+    __shared__ __align__(16) float2 sU[kScanWarps][kTS][K::CH];
+    __shared__ __align__(16) float sB[kScanWarps][kTS][K::NP];
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long wi = static_cast<long long>(blockIdx.x) * kScanWarps + w;
     if (wi >= warps) return;
-    const ScanPlace<NL> at = ScanPlace<NL>::of_warp(p, wi);
-    const int nl = lane % NL, cl = lane / NL, swap = nl & 1, n0 = nl * 4;
+    const ScanPlace at = ScanPlace::of_warp(p, wi, K::CH);
+    const int nl = lane % NL, cl = lane / NL, n0 = nl * 4;
     const int S = p.a.nstate, dim = p.a.dim;
     const int len = seq_len(p.a.lengths, at.b, p.a.length);
-    const int f0 = at.c0 + cl * kCT, fend = at.c0 + at.nc;
+    const int f = at.c0 + cl, ns = cl < at.nc ? min(max(S - n0, 0), 4) : 0;
     const int row = lane / K::LR, col = lane % K::LR * K::VX, bcol = lane % K::LR * K::VN;
     const int nx = min(max(at.nc - col, 0), K::VX), nb = min(max(S - bcol, 0), K::VN);
-    const long long out = static_cast<long long>(at.b) * p.nseg + at.seg;
-    St A2, h;
-    st_load(A2, p.a.A, f0, swap, fend, S, n0, p.vec_n);
+    St A2 = st_load(p.a.A, f, S, n0, ns, p.vec_n), h;
     st_scale(A2, kL2e);
     st_set(h, 0.f);
-    float sum[kCT] = {};
+    float sum = 0.f;
     const T* xp = static_cast<const T*>(REV ? p.a.dy : p.a.x) + at.b * (REV ? p.a.dy_batch : p.a.x_batch) + at.c0 + col;
     const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0 + col;
     const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0 + col;
@@ -173,10 +177,12 @@ __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP 
                   at.g * (REV ? p.a.C_group : p.a.B_group) + bcol;
     const long long x_time = REV ? p.a.dy_time : p.a.x_time, B_time = REV ? p.a.C_time : p.a.B_time;
     const bool vec_x = REV ? p.vec_dy : p.vec_x, vec_B = REV ? p.vec_C : p.vec_B;
-    const float* bias = p.a.delta_bias ? p.a.delta_bias + at.c0 + col : nullptr;
-    const int tend = min(at.t1, len), n = tend > at.t0 ? (tend - at.t0 + K::TS - 1) / K::TS : 0;
+    float bias[K::VX];
+#pragma unroll
+    for (int e = 0; e < K::VX; ++e) bias[e] = p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f;
+    const int tend = min(at.t1, len), n = tend > at.t0 ? (tend - at.t0 + kTS - 1) / kTS : 0;
     for (int k = 0; k < n; ++k) {
-        const int t = at.t0 + (REV ? n - 1 - k : k) * K::TS + row;
+        const int t = at.t0 + (REV ? n - 1 - k : k) * kTS + row;
         const bool in = t < len;
         Vec<T, K::VX> rx, rd, rz;
         Vec<T, K::VN> rB;
@@ -185,47 +191,38 @@ __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP 
         if (REV && p.a.z) rz.load_n(zp + t * p.a.z_time, in ? nx : 0, p.vec_z);
         rB.load_n(Bp + t * B_time, in ? nb : 0, vec_B);
         __syncwarp();
+        float v[2 * K::VX], b[K::VN];
 #pragma unroll
-        for (int e = 0; e < K::VX; e += 2) {
-            float dt[2], u[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                dt[q] = rd.get(e + q) + (bias && e + q < nx ? __ldg(bias + e + q) : 0.f);
-                if (p.a.softplus) dt[q] = softplusf(dt[q]);
-                if (!in) dt[q] = 0.f;
-                u[q] = rx.get(e + q);
-                if (!REV) u[q] *= dt[q];
-                if (REV && p.a.z) u[q] *= rz.get(e + q) * sigmoidf(rz.get(e + q));
-            }
-            sU[w][0][row][(col + e) / 2] = make_float4(dt[0], u[0], dt[1], u[1]);
-            sU[w][1][row][(col + e) / 2] = make_float4(dt[1], u[1], dt[0], u[0]);
+        for (int e = 0; e < K::VX; ++e) {
+            float dt = rd.get(e) + bias[e], u = rx.get(e);
+            if (p.a.softplus) dt = softplusf(dt);
+            if (!in) dt = 0.f;
+            if (!REV) u *= dt;
+            if (REV && p.a.z) u *= rz.get(e) * sigmoidf(rz.get(e));
+            v[2 * e] = dt;
+            v[2 * e + 1] = u;
         }
+        put_floats(reinterpret_cast<float*>(&sU[w][row][col]), v);
 #pragma unroll
-        for (int e = 0; e < K::VN; ++e) sB[w][row][bcol + e] = rB.get(e);
+        for (int e = 0; e < K::VN; ++e) b[e] = rB.get(e);
+        put_floats(&sB[w][row][bcol], b);
         __syncwarp();
 #pragma unroll 8
-        for (int i8 = 0; i8 < K::TS; ++i8) {
-            const int s = REV ? K::TS - 1 - i8 : i8;
-            const float4 du = sU[w][swap][s][cl];
+        for (int i = 0; i < kTS; ++i) {
+            const int s = REV ? kTS - 1 - i : i;
+            const float2 du = sU[w][s][cl];
             const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[w][s][n0]);
+            sum += du.x;
 #pragma unroll
-            for (int i = 0; i < kCT; ++i) {
-                const float dt = i ? du.z : du.x, u = i ? du.w : du.y;
-                sum[i] += dt;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const f2 a = ex22(mul2(pk(dt, dt), A2.v[i][j])), b{j ? bv.y : bv.x};
-                    h.v[i][j] = REV ? mul2(a, fma2(pk(u, u), b, h.v[i][j])) : fma2(a, h.v[i][j], mul2(pk(u, u), b));
-                }
+            for (int j = 0; j < 2; ++j) {
+                const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j])), u2 = pk(du.y, du.y);
+                h.v[j] = REV ? mul2(a, fma2(u2, half_of(bv, j), h.v[j])) : fma2(a, h.v[j], mul2(u2, half_of(bv, j)));
             }
         }
     }
-    st_store(h, p.seg_E + out * dim * S, f0, swap, fend, S, n0, p.vec_n);
-    if (nl == 0) {
-#pragma unroll
-        for (int i = 0; i < kCT; ++i)
-            if (f0 + i < fend) p.seg_dt[out * dim + f0 + i] = sum[i];
-    }
+    const long long orow = (static_cast<long long>(at.b) * p.nseg + at.seg) * dim + f;
+    st_store(h, p.seg_E, orow, S, n0, ns, p.vec_n);
+    if (nl == 0 && ns > 0) p.seg_dt[orow] = sum;
 }
 
 // One new step of every series: NL lanes per feature, 4 states each, read and
@@ -310,27 +307,26 @@ bool grid_of(long long warps, unsigned* blocks) {
 
 }  // namespace
 
-// Segments of the time axis: none while there are two warps per SM
-// sub-partition or nearly so; else enough for that, of 64 steps at least.
-ScanSplit scan_split(int batch, int length, int dim, int groups, int nstate, bool backward) {
-    const int nl = scan_lanes(nstate), ch = 32 / nl * kCT, ts = scan_stage_steps(nl), dg = dim / groups;
+// Segments of the time axis: none while there are enough warps for two per SM
+// sub-partition; else enough for that, of 64 steps at least and not more than 64
+// (every warp chains those before its own).
+ScanSplit scan_split(int batch, int length, int dim, int groups, int nstate) {
+    const int ch = 32 / scan_lanes(nstate), dg = dim / groups;
     const long long warps = static_cast<long long>(batch) * groups * ((dg + ch - 1) / ch);
-    (void)backward;
-    long long n = 1184 / warps;
-    n = std::min<long long>(n, length / 64);
+    long long n = 1776 / warps;
+    n = std::min<long long>(std::min<long long>(n, length / 64), 64);
     if (n < 3) n = 1;
     ScanSplit s;
-    s.seglen = static_cast<int>(((length + n - 1) / n + ts - 1) / ts * ts);
+    s.seglen = static_cast<int>(((length + n - 1) / n + kScanSave - 1) / kScanSave * kScanSave);
     s.nseg = (length + s.seglen - 1) / s.seglen;
     return s;
 }
 
 size_t scan_states(int batch, int length, int dim, int nstate) {
-    const int ts = scan_stage_steps(scan_lanes(nstate));
-    return static_cast<size_t>(batch) * ((length + ts - 1) / ts) * dim * nstate;
+    return static_cast<size_t>(batch) * ((length + kScanSave - 1) / kScanSave) * dim * nstate;
 }
 size_t scan_fwd_ws(int batch, int length, int dim, int groups, int nstate) {
-    return scan_segment_floats(batch, scan_split(batch, length, dim, groups, nstate, false).nseg, dim, nstate) * sizeof(float);
+    return scan_segment_floats(batch, scan_split(batch, length, dim, groups, nstate).nseg, dim, nstate) * sizeof(float);
 }
 
 cudaError_t launch_scan_segments(const ScanP& p, bool reverse, cudaStream_t st) {
@@ -354,7 +350,7 @@ cudaError_t launch_scan_fwd(const sdtw_scan_args& a, cudaStream_t st) {
         constexpr int NL = decltype(lanes)::value;
         ScanP p{};
         scan_params<T, NL>(p, a);
-        scan_segment_tables(p, scan_split(a.batch, a.length, a.dim, a.groups, a.nstate, false), a.workspace);
+        scan_segment_tables(p, scan_split(a.batch, a.length, a.dim, a.groups, a.nstate), a.workspace);
         const long long warps = static_cast<long long>(a.batch) * p.nseg * p.tiles_g * a.groups;
         unsigned blocks;
         if (!grid_of(warps, &blocks)) return cudaErrorInvalidConfiguration;
@@ -362,7 +358,8 @@ cudaError_t launch_scan_fwd(const sdtw_scan_args& a, cudaStream_t st) {
             const cudaError_t e = launch_scan_segments(p, false, st);
             if (e != cudaSuccess) return e;
         }
-        return launch_pdl(p.nseg > 1, scan_fwd_kernel<T, NL>, dim3(blocks), dim3(kScanThreads), 0, st, p, warps);
+        return launch_pdl(p.nseg > 1, p.full ? scan_fwd_kernel<T, NL, true> : scan_fwd_kernel<T, NL, false>, dim3(blocks),
+                          dim3(kScanThreads), 0, st, p, warps);
     });
 }
 

@@ -29,13 +29,12 @@ constexpr int scan_lanes(int nstate) {
     while (4 * nl < nstate) nl *= 2;
     return nl;
 }
-// Time steps staged at a time, which are also those between two stored states:
-// 16, or 8 for up to 8 states, whose tiles have more features.
-constexpr int scan_stage_steps(int lanes) { return lanes >= 4 ? 16 : 8; }
+// Time steps between two states that the forward stores for the backward.
+constexpr int kScanSave = 16;
 struct ScanSplit {
     int nseg, seglen;
 };
-ScanSplit scan_split(int batch, int length, int dim, int groups, int nstate, bool backward);
+ScanSplit scan_split(int batch, int length, int dim, int groups, int nstate);
 cudaError_t launch_scan_fwd(const sdtw_scan_args& a, cudaStream_t st);
 cudaError_t launch_scan_bwd(const sdtw_scan_args& a, cudaStream_t st);
 cudaError_t launch_scan_step(const sdtw_scan_args& a, cudaStream_t st);
