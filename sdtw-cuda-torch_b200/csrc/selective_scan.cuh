@@ -14,9 +14,13 @@
 // loads and multiply-adds): measured on B200 at 32 x 512 x 512, 16 states,
 // bfloat16, 120 us forward and 285 us backward that way.
 //
-// Time.  A warp walks over the time steps; dt, u, B and C of 16 steps at a time
-// are staged in shared memory, the elementwise functions computed once per
-// element there.  When there are too few warps to fill the GPU, the time axis is
+// Time.  A warp walks over the time steps, 16 staged in shared memory at a time:
+// the inputs as they are by asynchronous copies, which a piece ahead are on their
+// way during the work (loads to registers would hold the few scoreboards that
+// the inner loop needs), then dt and u, the elementwise functions computed once
+// per element.  B and C stay in the input's type until they are used: shared
+// memory moves 128 bytes a cycle whatever is read, and is what bounds the kernels.
+//  When there are too few warps to fill the GPU, the time axis is
 // cut into segments: a first kernel runs each from h = 0 and keeps its end state E
 // and the sum of its dt (whose exponential with A is the product of the decays),
 // and the main kernel's warps chain the segments before their own,
@@ -32,6 +36,7 @@ namespace sdtw {
 constexpr int kScanWarps = 4;
 constexpr int kScanThreads = 32 * kScanWarps;
 constexpr int kTS = kScanSave;  // staged time steps
+static_assert(kTS == 16, "two staging lanes per step");
 constexpr int kRun = 8;         // of them in registers at a time
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -52,7 +57,7 @@ struct ScanP {
     int nchunk;    // stored states per series
     int nseg, seglen;
     bool full;     // every tile has all its features and states, and every tensor its vector accesses
-    bool vec_x, vec_delta, vec_z, vec_B, vec_C, vec_y, vec_dy, vec_dx, vec_ddelta, vec_dz;
+    bool vec_y, vec_dx, vec_ddelta, vec_dz;
     bool vec_n;    // the states of a thread are 16 bytes aligned
     float* seg_dt;    // (batch, nseg, dim) sums of dt
     float* seg_E;     // (batch, nseg, dim, nstate) end states of the segments run from 0
@@ -104,7 +109,6 @@ __device__ __forceinline__ void st_store(const St& s, float* tab, long long row,
     for (int j = 0; j < 4; ++j) r.set(j, v[j]);
     r.store_n(tab + row * S + n0, n, vec);
 }
-__device__ __forceinline__ f2 half_of(ulonglong2 v, int j) { return f2{j ? v.y : v.x}; }
 // h <- exp(A sum dt) h + E over one segment.
 __device__ __forceinline__ void st_chain(St& h, const ScanP& p, const St& A2, int b, int seg, int f, int n0, int n) {
     const long long row = (static_cast<long long>(b) * p.nseg + seg) * p.a.dim + f;
@@ -114,16 +118,63 @@ __device__ __forceinline__ void st_chain(St& h, const ScanP& p, const St& A2, in
     for (int j = 0; j < 2; ++j) h.v[j] = fma2(ex22(mul2(pk(d, d), A2.v[j])), h.v[j], E.v[j]);
 }
 
-// Loads of a staging lane: n elements (0 or all of them when FULL).
-template <bool FULL, typename T, int V>
-__device__ __forceinline__ void stage_load(Vec<T, V>& r, const T* q, int n, bool vec) {
-    if constexpr (FULL) {
-        r.zero();
-        if (n > 0) r.load(q);
+// Four neighbouring values of B or C in shared memory as float pairs.
+template <typename T>
+__device__ __forceinline__ St quad(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+        return St{{f2{v.x}, f2{v.y}}};
     } else {
-        r.load_n(q, n, vec);
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        return St{{pk(half_bits<T>(v.x & 0xffffu), half_bits<T>(v.x >> 16)), pk(half_bits<T>(v.y & 0xffffu), half_bits<T>(v.y >> 16))}};
     }
 }
+
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// N bytes (4, 8 or 16) to shared memory, or zeros.
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool have) {
+    const int n = have ? N : 0;
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_addr(dst)), "l"(src), "n"(N), "r"(n) : "memory");
+}
+// Bytes of one copy of a row of W elements.
+template <typename T, int W>
+struct RowPiece {
+    static constexpr int kRow = W * static_cast<int>(sizeof(T));
+    static constexpr int kBytes = kRow < 16 ? (kRow < 4 ? 4 : kRow) : 16;
+    static constexpr int kElems = kBytes / static_cast<int>(sizeof(T));
+};
+// kTS rows of W elements, `time` elements apart in global memory, by one warp.
+// rows: how many of them exist, n: how many elements of a row (W when FULL); the
+// others become 0.  When FULL, or for 4-byte elements, the copies are under way
+// on return.
+template <bool FULL, typename T, int W>
+__device__ __forceinline__ void stage_rows(T* dst, const T* src, long long time, int rows, int n, int lane) {
+    if constexpr (FULL) {
+        using R = RowPiece<T, W>;
+        constexpr int per = W / R::kElems, total = kTS * per;
+#pragma unroll
+        for (int i0 = 0; i0 < total; i0 += 32) {
+            const int i = i0 + lane, r = i / per, c = i % per * R::kElems;
+            if (total % 32 == 0 || i < total) copy_async<R::kBytes>(dst + r * W + c, src + (r < rows ? r * time : 0) + c, r < rows);
+        }
+    } else {
+#pragma unroll
+        for (int i0 = 0; i0 < kTS * W; i0 += 32) {
+            const int i = i0 + lane, r = i / W, c = i % W;
+            const bool have = r < rows && c < n;
+            const T* q = src + (have ? r * time + c : 0);
+            if constexpr (sizeof(T) == 4)
+                copy_async<4>(dst + i, q, have);
+            else
+                reinterpret_cast<unsigned short*>(dst)[i] = have ? __ldg(reinterpret_cast<const unsigned short*>(q)) : 0;
+        }
+    }
+}
+// V values of a staging lane to global memory, n of them (0 or V when FULL).
 template <bool FULL, typename T, int V>
 __device__ __forceinline__ void stage_store(const Vec<T, V>& r, T* q, int n, bool vec) {
     if constexpr (FULL) {
@@ -172,22 +223,19 @@ inline void scan_params(ScanP& p, const sdtw_scan_args& a) {
     p.nchunk = (a.length + kScanSave - 1) / kScanSave;
     const bool d = p.dg % K::VX == 0;
     const long long ds = a.dim;
-    p.vec_x = d && vec_ok<T, K::VX>(a.x, a.x_batch, a.x_time);
-    p.vec_delta = d && vec_ok<T, K::VX>(a.delta, a.delta_batch, a.delta_time);
-    p.vec_z = d && vec_ok<T, K::VX>(a.z, a.z_batch, a.z_time);
     p.vec_y = d && vec_ok<T, K::VX>(a.y, ds, 0);
-    p.vec_dy = d && vec_ok<T, K::VX>(a.dy, a.dy_batch, a.dy_time);
     p.vec_dx = d && vec_ok<T, K::VX>(a.dx, ds, 0);
     p.vec_ddelta = d && vec_ok<T, K::VX>(a.ddelta, ds, 0);
     p.vec_dz = d && vec_ok<T, K::VX>(a.dz, ds, 0);
-    const bool n = a.nstate % K::VN == 0;
-    p.vec_B = n && vec_ok<T, K::VN>(a.B, a.B_batch, a.B_time, a.B_group);
-    p.vec_C = n && vec_ok<T, K::VN>(a.C, a.C_batch, a.C_time, a.C_group);
+    // Whole pieces of a staged row at multiples of the strides.
+    constexpr int PX = RowPiece<T, K::CH>::kElems, PN = RowPiece<T, K::NP>::kElems;
+    const bool rows = vec_ok<T, PX>(a.x, a.x_batch, a.x_time) && vec_ok<T, PX>(a.delta, a.delta_batch, a.delta_time) &&
+                      vec_ok<T, PX>(a.z, a.z_batch, a.z_time) && vec_ok<T, PX>(a.dy, a.dy_batch, a.dy_time) &&
+                      vec_ok<T, PN>(a.B, a.B_batch, a.B_time, a.B_group) && vec_ok<T, PN>(a.C, a.C_batch, a.C_time, a.C_group);
     p.vec_n = a.nstate % 4 == 0 && vec_ok<float, 4>(a.A, 0, 0) && vec_ok<float, 4>(a.state_in, a.state_in_batch, 0) &&
               vec_ok<float, 4>(a.state_out, a.state_out_batch, 0) && vec_ok<float, 4>(a.saved, 0, 0) &&
               vec_ok<float, 4>(a.dstate_in, 0, 0) && vec_ok<float, 4>(a.dstate_out, 0, 0);
-    p.full = p.dg % K::CH == 0 && a.nstate == K::NP && p.vec_x && p.vec_delta && p.vec_z && p.vec_y && p.vec_dy && p.vec_dx &&
-             p.vec_ddelta && p.vec_dz && p.vec_B && p.vec_C && p.vec_n;
+    p.full = rows && p.dg % K::CH == 0 && a.nstate == K::NP && p.vec_y && p.vec_dx && p.vec_ddelta && p.vec_dz && p.vec_n;
 }
 
 // The segments' tables at the start of a workspace, and their floats.

@@ -30,24 +30,32 @@
 namespace sdtw {
 namespace {
 
-template <int NL>
+// A warp's inputs of a piece, as they are; two of them, one on its way.
+template <typename T, int NL>
+struct alignas(16) BwdStage {
+    using K = ScanTile<NL>;
+    T x[kTS][K::CH], d[kTS][K::CH], g[kTS][K::CH], z[kTS][K::CH];
+};
+template <typename T, int NL>
 struct BwdSmem {
     using K = ScanTile<NL>;
     static constexpr int NQ = K::CH < 4 ? K::CH : 4;  // copies of B and C: states permuted by n ^ q within fours
-    float2 U[kScanWarps][kTS][K::CH];                 // (dt, u)
-    // Per element: gy; for the end of a piece x, softplus' and dout times the gate's derivative ...
-    float G[kScanWarps][kTS][K::CH], X[kScanWarps][kTS][K::CH], D[kScanWarps][kTS][K::CH], Z[kScanWarps][kTS][K::CH];
+    BwdStage<T, NL> in[kScanWarps][2];
+    // One more row than steps, so that the copies start in different banks.
+    alignas(16) T B[2][NQ][kTS + 1][K::NP];
+    alignas(16) T C[2][NQ][kTS + 1][K::NP];
+    alignas(16) float2 U[kScanWarps][kTS][K::CH];  // (dt, u)
+    // Per element: gy; for the end of a piece softplus' and dout times the gate's derivative ...
+    float G[kScanWarps][kTS][K::CH], D[kScanWarps][kTS][K::CH], Z[kScanWarps][kTS][K::CH];
     // ... and the sums q, s and y.
     float Q[kScanWarps][kTS][K::CH], R[kScanWarps][kTS][K::CH], Y[kScanWarps][kTS][K::CH];
-    // One more row than steps, so that the copies start in different banks.
-    float B[2][NQ][kTS + 1][K::NP], C[2][NQ][kTS + 1][K::NP];
     float acc[2][kScanWarps][kTS][2][K::NP];  // the warps' dB, dC
 };
 
 template <typename T, int NL, bool FULL>
 __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p) {
     using K = ScanTile<NL>;
-    using M = BwdSmem<NL>;
+    using M = BwdSmem<T, NL>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     M& sm = *reinterpret_cast<M*>(smem_raw);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -63,8 +71,8 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
     const int row = lane / K::LR, col = lane % K::LR * K::VX;
     const int nx = FULL ? (any ? K::VX : 0) : min(max(at.nc - col, 0), K::VX);
     const bool vn = FULL || p.vec_n;
-    // Staging of B and C: the block's 128 threads over the rows.
-    constexpr int BR = kScanThreads / kTS, BN = (K::NP + BR - 1) / BR;
+    // Staging of B and C: the block's 128 threads over the rows, neighbouring states in pairs.
+    constexpr int BR = kScanThreads / kTS, BN = (K::NP + BR - 1) / BR < 2 ? 2 : (K::NP + BR - 1) / BR;
     const int brow = threadIdx.x / BR, bcol = threadIdx.x % BR * BN;
 
     // States in this lane's order: register j holds state n0 + (j ^ perm).
@@ -101,48 +109,47 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
         skip[e] = p.a.D && e < nx ? __ldg(p.a.D + at.c0 + col + e) : 0.f;
     }
     const int tend = min(at.t1, len), pieces = tend > at.t0 ? (tend - at.t0 + kTS - 1) / kTS : 0;
-    // Pointers to the last piece; each fetch moves them one piece back.
-    const int tl = at.t0 + (pieces - 1) * kTS, rl = tl + row, bl = tl + brow;
-    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + rl * p.a.x_time + at.c0 + col;
-    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + rl * p.a.delta_time + at.c0 + col;
-    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + rl * p.a.z_time + at.c0 + col;
-    const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + rl * p.a.dy_time + at.c0 + col;
-    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + bl * p.a.B_time + at.g * p.a.B_group + bcol;
-    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + bl * p.a.C_time + at.g * p.a.C_group + bcol;
+    const int tl = at.t0 + (pieces - 1) * kTS;  // the last piece
+    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + at.c0;
+    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0;
+    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0;
+    const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + at.c0;
+    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + at.g * p.a.B_group + bcol;
+    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + at.g * p.a.C_group + bcol;
     const long long out0 = static_cast<long long>(at.b) * L * dim + at.c0 + col;
 
-    Vec<T, K::VX> rx, rd, rz, rg;
-    float nB[BN], nC[BN];
-    St hs;
-    auto fetch = [&](int tc) {
-        const int n = tc + row < len ? nx : 0;
-        stage_load<FULL>(rx, xp, n, p.vec_x);
-        stage_load<FULL>(rd, dp, n, p.vec_delta);
-        stage_load<FULL>(rg, gp, n, p.vec_dy);
-        if (p.a.z) stage_load<FULL>(rz, zp, n, p.vec_z);
-        const bool in = tc + brow < len;
-#pragma unroll
-        for (int e = 0; e < BN; ++e) {
-            const bool have = in && bcol + e < S;
-            nB[e] = have ? to_f(Bp[e]) : 0.f;
-            nC[e] = have ? to_f(Cp[e]) : 0.f;
-        }
-        hs = st_load(p.a.saved, (static_cast<long long>(at.b) * p.nchunk + tc / kScanSave) * dim + f, S, n0, ns, vn);
-        xp -= kTS * p.a.x_time;
-        dp -= kTS * p.a.delta_time;
-        gp -= kTS * p.a.dy_time;
-        zp -= kTS * p.a.z_time;
-        Bp -= kTS * p.a.B_time;
-        Cp -= kTS * p.a.C_time;
+    auto fetch = [&](int tc, BwdStage<T, NL>& st) {
+        const int rows = any ? min(tend - tc, kTS) : 0;
+        stage_rows<FULL, T, K::CH>(&st.x[0][0], xp + tc * p.a.x_time, p.a.x_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::CH>(&st.d[0][0], dp + tc * p.a.delta_time, p.a.delta_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::CH>(&st.g[0][0], gp + tc * p.a.dy_time, p.a.dy_time, rows, at.nc, lane);
+        if (p.a.z) stage_rows<FULL, T, K::CH>(&st.z[0][0], zp + tc * p.a.z_time, p.a.z_time, rows, at.nc, lane);
     };
+    Vec<T, BN> nB, nC;
+    St hs;
+    auto fetch_bc = [&](int tc) {
+        const int t = tc + brow, n = t < tend ? min(max(S - bcol, 0), BN) : 0;
+        nB.load_n(Bp + (n > 0 ? t * p.a.B_time : 0), n, false);
+        nC.load_n(Cp + (n > 0 ? t * p.a.C_time : 0), n, false);
+        hs = st_load(p.a.saved, (static_cast<long long>(at.b) * p.nchunk + tc / kScanSave) * dim + f, S, n0, ns, vn);
+    };
+    // Copy q holds state n at n ^ q: pairs change places with q / 2, and their halves with q % 2.
     auto stage_bc = [&](int buf) {
 #pragma unroll
-        for (int e = 0; e < BN; ++e)
+        for (int e = 0; e < BN; e += 2)
             if (bcol + e < K::NP) {
 #pragma unroll
                 for (int q = 0; q < M::NQ; ++q) {
-                    sm.B[buf][q][brow][(bcol + e) ^ q] = nB[e];
-                    sm.C[buf][q][brow][(bcol + e) ^ q] = nC[e];
+                    const int at_n = (bcol + e) ^ (q & 2);
+                    if constexpr (sizeof(T) == 2) {
+                        const int half = q & 1 ? 16 : 0;
+                        *reinterpret_cast<uint32_t*>(&sm.B[buf][q][brow][at_n]) = __funnelshift_r(nB.w[e / 2], nB.w[e / 2], half);
+                        *reinterpret_cast<uint32_t*>(&sm.C[buf][q][brow][at_n]) = __funnelshift_r(nC.w[e / 2], nC.w[e / 2], half);
+                    } else {
+                        const int a = q & 1;
+                        *reinterpret_cast<float2*>(&sm.B[buf][q][brow][at_n]) = make_float2(nB.get(e + a), nB.get(e + 1 - a));
+                        *reinterpret_cast<float2*>(&sm.C[buf][q][brow][at_n]) = make_float2(nC.get(e + a), nC.get(e + 1 - a));
+                    }
                 }
             }
     };
@@ -165,19 +172,27 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
     };
 
     if (pieces > 0) {
-        fetch(tl);
+        fetch(tl, sm.in[w][0]);
+        fetch_bc(tl);
         stage_bc(0);
     }
     for (int k = 0; k < pieces; ++k) {
         const int tc = tl - k * kTS, buf = k & 1, t = tc + row;
-        const bool in = t < len;
+        const bool in = t < tend;
+        BwdStage<T, NL>& st = sm.in[w][buf];
+        copy_async_wait();
         __syncwarp();
+        if (k + 1 < pieces) fetch(tc - kTS, sm.in[w][buf ^ 1]);
         {
-            float u[2 * K::VX], g[K::VX], x[K::VX], ds[K::VX], zf[K::VX];
+            Vec<T, K::VX> rx, rd, rz, rg;
+            rx.load_shared(&st.x[row][col]);
+            rd.load_shared(&st.d[row][col]);
+            rg.load_shared(&st.g[row][col]);
+            if (p.a.z) rz.load_shared(&st.z[row][col]);
+            float u[2 * K::VX], g[K::VX], ds[K::VX], zf[K::VX];
 #pragma unroll
             for (int e = 0; e < K::VX; ++e) {
                 float dt = rd.get(e) + bias[e];
-                x[e] = rx.get(e);
                 ds[e] = 1.f;
                 zf[e] = 0.f;
                 if (p.a.softplus) dt = softplusf(dt, &ds[e]);
@@ -189,11 +204,10 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
                     g[e] *= z * sg;
                 }
                 u[2 * e] = dt;
-                u[2 * e + 1] = dt * x[e];
+                u[2 * e + 1] = dt * rx.get(e);
             }
             put_floats(reinterpret_cast<float*>(&sm.U[w][row][col]), u);
             put_floats(&sm.G[w][row][col], g);
-            put_floats(&sm.X[w][row][col], x);
             put_floats(&sm.D[w][row][col], ds);
             put_floats(&sm.Z[w][row][col], zf);
         }
@@ -210,11 +224,11 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
 #pragma unroll
             for (int s = 0; s < kRun; ++s) {
                 const float2 du = sm.U[w][sb + s][cl];
-                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][perm][sb + s][n0]);
+                const St b = quad(&sm.B[buf][perm][sb + s][n0]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const f2 d = ex22(mul2(pk(du.x, du.x), A2.v[j]));
-                    s0.v[j] = fma2(d, s0.v[j], mul2(pk(du.y, du.y), half_of(bv, j)));
+                    s0.v[j] = fma2(d, s0.v[j], mul2(pk(du.y, du.y), b.v[j]));
                     if (keep) {
                         a[s][j] = d;
                         h[s][j] = s0.v[j];
@@ -236,14 +250,13 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
             for (int s = kRun - 1; s >= 0; --s) {
                 const float2 du = sm.U[w][sb + s][cl];
                 const float gy = sm.G[w][sb + s][cl];
-                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][perm][sb + s][n0]);
-                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sm.C[buf][perm][sb + s][n0]);
+                const St b = quad(&sm.B[buf][perm][sb + s][n0]), c = quad(&sm.C[buf][perm][sb + s][n0]);
                 const f2 g2 = pk(gy, gy), u2 = pk(du.y, du.y), d2 = pk(du.x, du.x);
                 float vb[4], vc[4];
                 f2 q, sa, y;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const f2 b2 = half_of(bv, j), c2 = half_of(cv, j);
+                    const f2 b2 = b.v[j], c2 = c.v[j];
                     const f2 gh = fma2(g2, c2, r.v[j]);
                     r.v[j] = mul2(a[s][j], gh);
                     const f2 kk = mul2(r.v[j], s > 0 ? h[s > 0 ? s - 1 : 0][j] : hin.v[j]);
@@ -301,20 +314,21 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
                 }
             }
         }
-        if (k + 1 < pieces) {  // on their way during what follows
-            fetch(tc - kTS);
-        }
+        if (k + 1 < pieces) fetch_bc(tc - kTS);  // on their way during what follows
         __syncwarp();
         {
+            Vec<T, K::VX> rx;
+            rx.load_shared(&st.x[row][col]);
             float u[2 * K::VX], g[K::VX], x[K::VX], ds[K::VX], zf[K::VX], q[K::VX], sr[K::VX], y[K::VX];
             get_floats(u, reinterpret_cast<const float*>(&sm.U[w][row][col]));
             get_floats(g, &sm.G[w][row][col]);
-            get_floats(x, &sm.X[w][row][col]);
             get_floats(ds, &sm.D[w][row][col]);
             get_floats(zf, &sm.Z[w][row][col]);
             get_floats(q, &sm.Q[w][row][col]);
             get_floats(sr, &sm.R[w][row][col]);
             get_floats(y, &sm.Y[w][row][col]);
+#pragma unroll
+            for (int e = 0; e < K::VX; ++e) x[e] = rx.get(e);
             Vec<T, K::VX> ox, od, oz;
 #pragma unroll
             for (int e = 0; e < K::VX; ++e) {
@@ -332,6 +346,7 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
             if (p.a.z && p.a.dz) stage_store<FULL>(oz, static_cast<T*>(p.a.dz) + o, no, p.vec_dz);
         }
         if (k + 1 < pieces) stage_bc(buf ^ 1);  // read last a piece ago, before this piece's barrier
+        __syncwarp();
     }
     for (int t = at.t0 + pieces * kTS + row; t < at.t1; t += kTS) {
         Vec<T, K::VX> o;
@@ -429,7 +444,7 @@ cudaError_t run_scan_bwd(const sdtw_scan_args& a, cudaStream_t st) {
     const long long nbc = (static_cast<long long>(a.batch) * a.length * a.groups * 2 * 4 * NL + 255) / 256;
     const long long npar = (static_cast<long long>(a.dim) * (a.nstate + 2) + 255) / 256;
     if (blocks > 0x7fffffffll || nbc + npar > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    const int smem = static_cast<int>(sizeof(BwdSmem<NL>));
+    const int smem = static_cast<int>(sizeof(BwdSmem<T, NL>));
     const auto kernel = p.full ? scan_bwd_kernel<T, NL, true> : scan_bwd_kernel<T, NL, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;

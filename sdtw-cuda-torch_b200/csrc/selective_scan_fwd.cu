@@ -8,13 +8,27 @@
 namespace sdtw {
 namespace {
 
+// A warp's inputs of a piece, as they are; two of them, one on its way.
+template <typename T, int NL>
+struct alignas(16) FwdStage {
+    using K = ScanTile<NL>;
+    T x[kTS][K::CH], d[kTS][K::CH], z[kTS][K::CH], B[kTS][K::NP], C[kTS][K::NP];
+};
+template <typename T, int NL>
+struct FwdSmem {
+    using K = ScanTile<NL>;
+    FwdStage<T, NL> in[kScanWarps][2];
+    alignas(16) float2 U[kScanWarps][kTS][K::CH];  // (dt, u)
+    float Y[kScanWarps][kTS][K::CH];
+};
+
 // One warp per (series, segment, tile of features); the warps of a block do not
 // wait for one another.
 template <typename T, int NL, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 3) scan_fwd_kernel(const ScanP p, long long warps) {
+__global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanP p, long long warps) {
     using K = ScanTile<NL>;
-    __shared__ __align__(16) float2 sU[kScanWarps][kTS][K::CH];  // (dt, u)
-    __shared__ __align__(16) float sB[kScanWarps][kTS][K::NP], sC[kScanWarps][kTS][K::NP], sY[kScanWarps][kTS][K::CH];
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    FwdSmem<T, NL>& sm = *reinterpret_cast<FwdSmem<T, NL>*>(smem_raw);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long wi = static_cast<long long>(blockIdx.x) * kScanWarps + w;
     if (wi >= warps) return;
@@ -23,8 +37,8 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
     const int S = p.a.nstate, L = p.a.length, dim = p.a.dim;
     const int len = seq_len(p.a.lengths, at.b, L);
     const int f = at.c0 + cl, ns = FULL ? 4 : (cl < at.nc ? min(max(S - n0, 0), 4) : 0);
-    const int row = lane / K::LR, col = lane % K::LR * K::VX, bcol = lane % K::LR * K::VN;
-    const int nx = FULL ? K::VX : min(max(at.nc - col, 0), K::VX), nb = FULL ? K::VN : min(max(S - bcol, 0), K::VN);
+    const int row = lane / K::LR, col = lane % K::LR * K::VX;
+    const int nx = FULL ? K::VX : min(max(at.nc - col, 0), K::VX);
     const bool vn = FULL || p.vec_n;
 
     St A2 = st_load(p.a.A, f, S, n0, ns, vn), h;
@@ -42,43 +56,37 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
         bias[e] = p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f;
         skip[e] = p.a.D && e < nx ? __ldg(p.a.D + at.c0 + col + e) : 0.f;
     }
-    const int r0 = at.t0 + row;  // the first step that this lane stages
-    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + r0 * p.a.x_time + at.c0 + col;
-    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + r0 * p.a.delta_time + at.c0 + col;
-    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + r0 * p.a.z_time + at.c0 + col;
-    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + r0 * p.a.B_time + at.g * p.a.B_group + bcol;
-    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + r0 * p.a.C_time + at.g * p.a.C_group + bcol;
-    T* yp = static_cast<T*>(p.a.y) + (static_cast<long long>(at.b) * L + r0) * dim + at.c0 + col;
+    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + at.c0;
+    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0;
+    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0;
+    const T* Bp = static_cast<const T*>(p.a.B) + at.b * p.a.B_batch + at.g * p.a.B_group;
+    const T* Cp = static_cast<const T*>(p.a.C) + at.b * p.a.C_batch + at.g * p.a.C_group;
+    T* yp = static_cast<T*>(p.a.y) + (static_cast<long long>(at.b) * L + at.t0 + row) * dim + at.c0 + col;
     float* sp = p.a.saved ? p.a.saved + (static_cast<long long>(at.b) * p.nchunk + at.t0 / kScanSave) * dim * S : nullptr;
-
-    Vec<T, K::VX> rx, rd;
-    Vec<T, K::VN> rB, rC;
-    auto fetch = [&](int t) {
-        const bool in = t < len;
-        stage_load<FULL>(rx, xp, in ? nx : 0, p.vec_x);
-        stage_load<FULL>(rd, dp, in ? nx : 0, p.vec_delta);
-        stage_load<FULL>(rB, Bp, in ? nb : 0, p.vec_B);
-        stage_load<FULL>(rC, Cp, in ? nb : 0, p.vec_C);
-        xp += kTS * p.a.x_time;
-        dp += kTS * p.a.delta_time;
-        Bp += kTS * p.a.B_time;
-        Cp += kTS * p.a.C_time;
-    };
     const int tend = min(at.t1, len);
-    if (at.t0 < tend) fetch(r0);
-    int tc = at.t0;
-    for (; tc < tend; tc += kTS) {
+    auto fetch = [&](int tc, FwdStage<T, NL>& st) {
+        const int rows = min(tend - tc, kTS);
+        stage_rows<FULL, T, K::CH>(&st.x[0][0], xp + tc * p.a.x_time, p.a.x_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::CH>(&st.d[0][0], dp + tc * p.a.delta_time, p.a.delta_time, rows, at.nc, lane);
+        if (p.a.z) stage_rows<FULL, T, K::CH>(&st.z[0][0], zp + tc * p.a.z_time, p.a.z_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::NP>(&st.B[0][0], Bp + tc * p.a.B_time, p.a.B_time, rows, S, lane);
+        stage_rows<FULL, T, K::NP>(&st.C[0][0], Cp + tc * p.a.C_time, p.a.C_time, rows, S, lane);
+    };
+    if (at.t0 < tend) fetch(at.t0, sm.in[w][0]);
+    int tc = at.t0, buf = 0;
+    for (; tc < tend; tc += kTS, buf ^= 1) {
         const int t = tc + row;
-        const bool in = t < len;
-        const Vec<T, K::VX> xk = rx;
-        Vec<T, K::VX> rz;
-        if (p.a.z) {
-            stage_load<FULL>(rz, zp, in ? nx : 0, p.vec_z);
-            zp += kTS * p.a.z_time;
-        }
+        const bool in = t < tend;
+        FwdStage<T, NL>& st = sm.in[w][buf];
+        copy_async_wait();
         __syncwarp();
+        if (tc + kTS < tend) fetch(tc + kTS, sm.in[w][buf ^ 1]);
+        Vec<T, K::VX> rx;
+        rx.load_shared(&st.x[row][col]);
         {
-            float v[2 * K::VX], b[K::VN], c[K::VN];
+            Vec<T, K::VX> rd;
+            rd.load_shared(&st.d[row][col]);
+            float v[2 * K::VX];
 #pragma unroll
             for (int e = 0; e < K::VX; ++e) {
                 float dt = rd.get(e) + bias[e];
@@ -87,16 +95,8 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
                 v[2 * e] = dt;
                 v[2 * e + 1] = dt * rx.get(e);
             }
-            put_floats(reinterpret_cast<float*>(&sU[w][row][col]), v);
-#pragma unroll
-            for (int e = 0; e < K::VN; ++e) {
-                b[e] = rB.get(e);
-                c[e] = rC.get(e);
-            }
-            put_floats(&sB[w][row][bcol], b);
-            put_floats(&sC[w][row][bcol], c);
+            put_floats(reinterpret_cast<float*>(&sm.U[w][row][col]), v);
         }
-        if (tc + kTS < tend) fetch(t + kTS);
         __syncwarp();
         if (sp) {
             st_store(h, sp, f, S, n0, ns, vn);
@@ -107,31 +107,31 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
             float v[kRun];
 #pragma unroll
             for (int s = 0; s < kRun; ++s) {
-                const float2 du = sU[w][sb + s][cl];
-                const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[w][sb + s][n0]);
-                const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(&sC[w][sb + s][n0]);
+                const float2 du = sm.U[w][sb + s][cl];
+                const St b = quad(&st.B[sb + s][n0]), c = quad(&st.C[sb + s][n0]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j]));
-                    h.v[j] = fma2(a, h.v[j], mul2(pk(du.y, du.y), half_of(bv, j)));
+                    h.v[j] = fma2(a, h.v[j], mul2(pk(du.y, du.y), b.v[j]));
                 }
-                v[s] = sum2(fma2(half_of(cv, 1), h.v[1], mul2(half_of(cv, 0), h.v[0])));
+                v[s] = sum2(fma2(c.v[1], h.v[1], mul2(c.v[0], h.v[0])));
             }
             using Sum = LaneSum<kRun, 1, NL>;
             Sum::run(v, lane);
             if (Sum::owner(lane)) {
                 const int slot = Sum::slot(lane);
 #pragma unroll
-                for (int k = 0; k < Sum::kept; ++k) sY[w][sb + slot + k][cl] = v[k];
+                for (int k = 0; k < Sum::kept; ++k) sm.Y[w][sb + slot + k][cl] = v[k];
             }
         }
         __syncwarp();
         float y[K::VX];
-        get_floats(y, &sY[w][row][col]);
-        Vec<T, K::VX> o;
+        get_floats(y, &sm.Y[w][row][col]);
+        Vec<T, K::VX> rz, o;
+        if (p.a.z) rz.load_shared(&st.z[row][col]);
 #pragma unroll
         for (int e = 0; e < K::VX; ++e) {
-            y[e] = fmaf(skip[e], xk.get(e), y[e]);
+            y[e] = fmaf(skip[e], rx.get(e), y[e]);
             if (p.a.z) {
                 const float z = rz.get(e);
                 y[e] *= z * sigmoidf(z);
@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
         }
         stage_store<FULL>(o, yp, t < at.t1 ? nx : 0, p.vec_y);
         yp += static_cast<long long>(kTS) * dim;
+        __syncwarp();  // before the next piece but one comes into this one's place
     }
     for (int t = tc + row; t < at.t1; t += kTS) {
         Vec<T, K::VX> o;
@@ -151,11 +152,11 @@ __global__ void __launch_bounds__(kScanThreads, NL == 4 && sizeof(T) == 2 ? 4 : 
 }
 
 // End state and sum of dt of a segment run from 0: see launch_scan_segments.
-template <typename T, int NL, bool REV>
+template <typename T, int NL, bool REV, bool FULL>
 __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP p, long long warps) {
     using K = ScanTile<NL>;
-    __shared__ __align__(16) float2 sU[kScanWarps][kTS][K::CH];
-    __shared__ __align__(16) float sB[kScanWarps][kTS][K::NP];
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    FwdSmem<T, NL>& sm = *reinterpret_cast<FwdSmem<T, NL>*>(smem_raw);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long wi = static_cast<long long>(blockIdx.x) * kScanWarps + w;
     if (wi >= warps) return;
@@ -164,34 +165,42 @@ __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP 
     const int S = p.a.nstate, dim = p.a.dim;
     const int len = seq_len(p.a.lengths, at.b, p.a.length);
     const int f = at.c0 + cl, ns = cl < at.nc ? min(max(S - n0, 0), 4) : 0;
-    const int row = lane / K::LR, col = lane % K::LR * K::VX, bcol = lane % K::LR * K::VN;
-    const int nx = min(max(at.nc - col, 0), K::VX), nb = min(max(S - bcol, 0), K::VN);
+    const int row = lane / K::LR, col = lane % K::LR * K::VX;
+    const int nx = min(max(at.nc - col, 0), K::VX);
     St A2 = st_load(p.a.A, f, S, n0, ns, p.vec_n), h;
     st_scale(A2, kL2e);
     st_set(h, 0.f);
     float sum = 0.f;
-    const T* xp = static_cast<const T*>(REV ? p.a.dy : p.a.x) + at.b * (REV ? p.a.dy_batch : p.a.x_batch) + at.c0 + col;
-    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0 + col;
-    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0 + col;
+    const T* xp = static_cast<const T*>(REV ? p.a.dy : p.a.x) + at.b * (REV ? p.a.dy_batch : p.a.x_batch) + at.c0;
+    const T* dp = static_cast<const T*>(p.a.delta) + at.b * p.a.delta_batch + at.c0;
+    const T* zp = static_cast<const T*>(p.a.z) + at.b * p.a.z_batch + at.c0;
     const T* Bp = static_cast<const T*>(REV ? p.a.C : p.a.B) + at.b * (REV ? p.a.C_batch : p.a.B_batch) +
-                  at.g * (REV ? p.a.C_group : p.a.B_group) + bcol;
+                  at.g * (REV ? p.a.C_group : p.a.B_group);
     const long long x_time = REV ? p.a.dy_time : p.a.x_time, B_time = REV ? p.a.C_time : p.a.B_time;
-    const bool vec_x = REV ? p.vec_dy : p.vec_x, vec_B = REV ? p.vec_C : p.vec_B;
     float bias[K::VX];
 #pragma unroll
     for (int e = 0; e < K::VX; ++e) bias[e] = p.a.delta_bias && e < nx ? __ldg(p.a.delta_bias + at.c0 + col + e) : 0.f;
     const int tend = min(at.t1, len), n = tend > at.t0 ? (tend - at.t0 + kTS - 1) / kTS : 0;
+    auto start_of = [&](int k) { return at.t0 + (REV ? n - 1 - k : k) * kTS; };
+    auto fetch = [&](int tc, FwdStage<T, NL>& st) {
+        const int rows = min(tend - tc, kTS);
+        stage_rows<FULL, T, K::CH>(&st.x[0][0], xp + tc * x_time, x_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::CH>(&st.d[0][0], dp + tc * p.a.delta_time, p.a.delta_time, rows, at.nc, lane);
+        if (REV && p.a.z) stage_rows<FULL, T, K::CH>(&st.z[0][0], zp + tc * p.a.z_time, p.a.z_time, rows, at.nc, lane);
+        stage_rows<FULL, T, K::NP>(&st.B[0][0], Bp + tc * B_time, B_time, rows, S, lane);
+    };
+    if (n > 0) fetch(start_of(0), sm.in[w][0]);
     for (int k = 0; k < n; ++k) {
-        const int t = at.t0 + (REV ? n - 1 - k : k) * kTS + row;
-        const bool in = t < len;
-        Vec<T, K::VX> rx, rd, rz;
-        Vec<T, K::VN> rB;
-        rx.load_n(xp + t * x_time, in ? nx : 0, vec_x);
-        rd.load_n(dp + t * p.a.delta_time, in ? nx : 0, p.vec_delta);
-        if (REV && p.a.z) rz.load_n(zp + t * p.a.z_time, in ? nx : 0, p.vec_z);
-        rB.load_n(Bp + t * B_time, in ? nb : 0, vec_B);
+        const bool in = start_of(k) + row < tend;
+        FwdStage<T, NL>& st = sm.in[w][k & 1];
+        copy_async_wait();
         __syncwarp();
-        float v[2 * K::VX], b[K::VN];
+        if (k + 1 < n) fetch(start_of(k + 1), sm.in[w][(k & 1) ^ 1]);
+        Vec<T, K::VX> rx, rd, rz;
+        rx.load_shared(&st.x[row][col]);
+        rd.load_shared(&st.d[row][col]);
+        if (REV && p.a.z) rz.load_shared(&st.z[row][col]);
+        float v[2 * K::VX];
 #pragma unroll
         for (int e = 0; e < K::VX; ++e) {
             float dt = rd.get(e) + bias[e], u = rx.get(e);
@@ -202,23 +211,21 @@ __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP 
             v[2 * e] = dt;
             v[2 * e + 1] = u;
         }
-        put_floats(reinterpret_cast<float*>(&sU[w][row][col]), v);
-#pragma unroll
-        for (int e = 0; e < K::VN; ++e) b[e] = rB.get(e);
-        put_floats(&sB[w][row][bcol], b);
+        put_floats(reinterpret_cast<float*>(&sm.U[w][row][col]), v);
         __syncwarp();
 #pragma unroll 8
         for (int i = 0; i < kTS; ++i) {
             const int s = REV ? kTS - 1 - i : i;
-            const float2 du = sU[w][s][cl];
-            const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(&sB[w][s][n0]);
+            const float2 du = sm.U[w][s][cl];
+            const St b = quad(&st.B[s][n0]);
             sum += du.x;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j])), u2 = pk(du.y, du.y);
-                h.v[j] = REV ? mul2(a, fma2(u2, half_of(bv, j), h.v[j])) : fma2(a, h.v[j], mul2(u2, half_of(bv, j)));
+                h.v[j] = REV ? mul2(a, fma2(u2, b.v[j], h.v[j])) : fma2(a, h.v[j], mul2(u2, b.v[j]));
             }
         }
+        __syncwarp();
     }
     const long long orow = (static_cast<long long>(at.b) * p.nseg + at.seg) * dim + f;
     st_store(h, p.seg_E, orow, S, n0, ns, p.vec_n);
@@ -336,11 +343,12 @@ cudaError_t launch_scan_segments(const ScanP& p, bool reverse, cudaStream_t st) 
         const long long warps = static_cast<long long>(p.a.batch) * p.nseg * p.tiles_g * p.a.groups;
         unsigned blocks;
         if (!grid_of(warps, &blocks)) return cudaErrorInvalidConfiguration;
-        if (reverse)
-            scan_segment_kernel<T, NL, true><<<blocks, kScanThreads, 0, st>>>(p, warps);
-        else
-            scan_segment_kernel<T, NL, false><<<blocks, kScanThreads, 0, st>>>(p, warps);
-        return cudaGetLastError();
+        const auto kernel = reverse ? (p.full ? scan_segment_kernel<T, NL, true, true> : scan_segment_kernel<T, NL, true, false>)
+                                    : (p.full ? scan_segment_kernel<T, NL, false, true> : scan_segment_kernel<T, NL, false, false>);
+        constexpr int smem = sizeof(FwdSmem<T, NL>);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(false, kernel, dim3(blocks), dim3(kScanThreads), smem, st, p, warps);
     });
 }
 
@@ -358,8 +366,11 @@ cudaError_t launch_scan_fwd(const sdtw_scan_args& a, cudaStream_t st) {
             const cudaError_t e = launch_scan_segments(p, false, st);
             if (e != cudaSuccess) return e;
         }
-        return launch_pdl(p.nseg > 1, p.full ? scan_fwd_kernel<T, NL, true> : scan_fwd_kernel<T, NL, false>, dim3(blocks),
-                          dim3(kScanThreads), 0, st, p, warps);
+        const auto kernel = p.full ? scan_fwd_kernel<T, NL, true> : scan_fwd_kernel<T, NL, false>;
+        constexpr int smem = sizeof(FwdSmem<T, NL>);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(p.nseg > 1, kernel, dim3(blocks), dim3(kScanThreads), smem, st, p, warps);
     });
 }
 

@@ -102,6 +102,27 @@ struct Vec {
             *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(w[0]);
         }
     }
+    // From shared memory, aligned for whole pieces.
+    __device__ __forceinline__ void load_shared(const T* p) {
+        if constexpr (kPiece == 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i) {
+                const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = q.x;
+                w[4 * i + 1] = q.y;
+                w[4 * i + 2] = q.z;
+                w[4 * i + 3] = q.w;
+            }
+        } else if constexpr (kPiece == 8) {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            w[0] = q.x;
+            w[1] = q.y;
+        } else if constexpr (kPiece == 4) {
+            w[0] = *reinterpret_cast<const unsigned int*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const unsigned short*>(p);
+        }
+    }
     // n of the V elements exist at p (the others read as 0); `vec`: p is
     // aligned for whole pieces and n is 0 or V.
     __device__ __forceinline__ void load_n(const T* p, int n, bool vec) {
