@@ -32,6 +32,7 @@ struct ConvP {
     int nchb;    // blocks over features
     int ntb;     // blocks over time
     bool vec_x, vec_y, vec_s, vec_so, vec_dy, vec_dx, vec_dso;
+    bool full;   // every access of x, y, dy and dx is a whole vector
     float* part;
 };
 
@@ -123,7 +124,24 @@ struct ConvPlace {
     }
 };
 
-template <typename T, int VEC, int WT>
+template <bool FULL, typename T, int VEC>
+__device__ __forceinline__ void load_step(Vec<T, VEC>& r, const T* q, bool have, int n, bool vec) {
+    if constexpr (FULL) {
+        r.zero();
+        if (have) r.load(q);
+    } else {
+        r.load_n(q, have ? n : 0, vec);
+    }
+}
+template <bool FULL, typename T, int VEC>
+__device__ __forceinline__ void store_step(const Vec<T, VEC>& r, T* q, int n, bool vec) {
+    if constexpr (FULL)
+        r.store(q);
+    else
+        r.store_n(q, n, vec);
+}
+
+template <typename T, int VEC, int WT, bool FULL>
 __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
     constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 8;
     const int W = Width<WT>::get(p.a.width);
@@ -140,13 +158,16 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
         if (m < W) load_s<T, VEC>(p, at.b, c, n, at.t0 + W - 1 - m, W, at.len, r);
         to_pairs<T, VEC>(r, xs[KM - 1 - m]);
     }
-    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + c;
-    T* yp = static_cast<T*>(p.a.y) + static_cast<long long>(at.b) * p.a.length * p.a.dim + c;
+    const long long xt = p.a.x_time, yt = p.a.dim;
+    const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + at.t0 * xt + c;
+    T* yp = static_cast<T*>(p.a.y) + (static_cast<long long>(at.b) * p.a.length + at.t0) * yt + c;
     const int tl = min(at.t1, at.len);
     Vec<T, VEC> next[U];
     auto fetch = [&](int t) {
+        const T* q = xp;
 #pragma unroll
-        for (int u = 0; u < U; ++u) next[u].load_n(xp + (t + u) * p.a.x_time, t + u < tl ? n : 0, p.vec_x);
+        for (int u = 0; u < U; ++u, q += xt) load_step<FULL>(next[u], q, t + u < tl, n, p.vec_x);
+        xp = q;
     };
     fetch(at.t0);
     for (int t = at.t0; t < at.t1; t += U) {
@@ -154,23 +175,24 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
         for (int u = 0; u < U; ++u) to_pairs<T, VEC>(next[u], xs[KM - 1 + u]);
         if (t + U < at.t1) fetch(t + U);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Vec<T, VEC> o;
+        for (int u = 0; u < U; ++u, yp += yt) {
+            float y[VEC];
 #pragma unroll
             for (int q = 0; q < VP; ++q) {
                 f2 v = k.bias[q];
 #pragma unroll
                 for (int m = 0; m < KM; ++m)
                     if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
-                float y[2];
-                upk(v, y[0], y[1]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (p.a.silu) y[e] *= sigmoidf(y[e]);
-                    o.set(2 * q + e, t + u < at.len ? y[e] : 0.f);
-                }
+                upk(v, y[2 * q], y[2 * q + 1]);
             }
-            if (t + u < at.t1) o.store_n(yp + static_cast<long long>(t + u) * p.a.dim, n, p.vec_y);
+            if (p.a.silu) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) y[e] *= sigmoidf(y[e]);
+            }
+            Vec<T, VEC> o;
+            o.put(y);
+            if (t + u >= at.len) o.zero();
+            if (t + u < at.t1) store_step<FULL>(o, yp, n, p.vec_y);
         }
 #pragma unroll
         for (int m = 0; m < KM - 1; ++m)
@@ -186,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
     }
 }
 
-template <typename T, int VEC, int WT>
+template <typename T, int VEC, int WT, bool FULL>
 __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
     constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 4;
     const int W = Width<WT>::get(p.a.width);
@@ -213,19 +235,20 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
 #pragma unroll
             for (int q = 0; q < VP; ++q) gs[KM - 1 - m][q] = pk(0.f, 0.f);
         }
-        const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + c;
-        const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + c;
-        T* dxp = static_cast<T*>(p.a.dx) + static_cast<long long>(at.b) * p.a.length * p.a.dim + c;
+        const long long xt = p.a.x_time, gt = p.a.dy_time, dt = p.a.dim;
+        const T* xp = static_cast<const T*>(p.a.x) + at.b * p.a.x_batch + t0 * xt + c;
+        const T* gp = static_cast<const T*>(p.a.dy) + at.b * p.a.dy_batch + t0 * gt + c;
+        // Where step t0's x[t0 - (W - 1)] would be; stored to from t0 on only.
+        T* dxp = static_cast<T*>(p.a.dx) + (static_cast<long long>(at.b) * p.a.length + t0 - (W - 1)) * dt + c;
         // Step j brings gv[j] and with it dL/ds[j], which is the gradient of
         // x[j - (W - 1)]; the W - 1 steps behind the tile complete its last ones.
         const int j_end = t1 + W - 1, jl = min(j_end, len);
         Vec<T, VEC> nx[U], ng[U];
         auto fetch = [&](int j) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int m = j + u < jl ? n : 0;
-                nx[u].load_n(xp + (j + u) * p.a.x_time, m, p.vec_x);
-                ng[u].load_n(gp + (j + u) * p.a.dy_time, m, p.vec_dy);
+            for (int u = 0; u < U; ++u, xp += xt, gp += gt) {
+                load_step<FULL>(nx[u], xp, j + u < jl, n, p.vec_x);
+                load_step<FULL>(ng[u], gp, j + u < jl, n, p.vec_dy);
             }
         };
         fetch(t0);
@@ -237,45 +260,46 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
             }
             if (j0 + U < j_end) fetch(j0 + U);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u, dxp += dt) {
                 const int j = j0 + u, t = j - (W - 1);
-                const bool own = j < t1;
-                float ds[VEC];
+                if (p.a.silu) {  // gv = dy times the derivative; dy is 0 from the valid steps' end on
 #pragma unroll
-                for (int q = 0; q < VP; ++q) {
-                    f2 g = gs[KM - 1 + u][q];
-                    if (p.a.silu) {
+                    for (int q = 0; q < VP; ++q) {
                         f2 v = k.bias[q];
 #pragma unroll
                         for (int m = 0; m < KM; ++m)
                             if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
                         float a, b;
                         upk(v, a, b);
-                        g = mul2(g, pk(dsilu(a), dsilu(b)));
+                        gs[KM - 1 + u][q] = mul2(gs[KM - 1 + u][q], pk(dsilu(a), dsilu(b)));
                     }
-                    if (j >= len) g = pk(0.f, 0.f);
-                    gs[KM - 1 + u][q] = g;
-                    if (own) {
-                        db[q] = add2(db[q], g);
+                }
+                if (j < t1) {
+#pragma unroll
+                    for (int q = 0; q < VP; ++q) {
+                        db[q] = add2(db[q], gs[KM - 1 + u][q]);
 #pragma unroll
                         for (int m = 0; m < KM; ++m)
-                            if (m < W) dw[m][q] = fma2(g, xs[KM - 1 + u - m][q], dw[m][q]);
+                            if (m < W) dw[m][q] = fma2(gs[KM - 1 + u][q], xs[KM - 1 + u - m][q], dw[m][q]);
                     }
-                    // sum_k w[k] gv[j - k], w[k] = wr[W - 1 - k].
-                    f2 d = pk(0.f, 0.f);
-                    if constexpr (WT != 0) {
-#pragma unroll
-                        for (int i = 0; i < KM; ++i) d = fma2(k.wr[KM - 1 - i][q], gs[KM - 1 + u - i][q], d);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < KM; ++i)
-#pragma unroll
-                            for (int m = 0; m < KM; ++m)
-                                if (m + i == W - 1) d = fma2(k.wr[m][q], gs[KM - 1 + u - i][q], d);
-                    }
-                    upk(d, ds[2 * q], ds[2 * q + 1]);
                 }
                 if (p.a.dx && t >= t0 && t < t1) {
+                    float ds[VEC];
+#pragma unroll
+                    for (int q = 0; q < VP; ++q) {  // sum_k w[k] gv[j - k], w[k] = wr[W - 1 - k]
+                        f2 d = pk(0.f, 0.f);
+                        if constexpr (WT != 0) {
+#pragma unroll
+                            for (int i = 0; i < KM; ++i) d = fma2(k.wr[KM - 1 - i][q], gs[KM - 1 + u - i][q], d);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < KM; ++i)
+#pragma unroll
+                                for (int m = 0; m < KM; ++m)
+                                    if (m + i == W - 1) d = fma2(k.wr[m][q], gs[KM - 1 + u - i][q], d);
+                        }
+                        upk(d, ds[2 * q], ds[2 * q + 1]);
+                    }
                     if (p.a.dstate_out && t < len && j >= len) {
                         Vec<T, VEC> r;
                         r.load_n(static_cast<const T*>(p.a.dstate_out) + (static_cast<long long>(at.b) * (W - 1) + (j - len)) * p.a.dim + c, n,
@@ -284,9 +308,9 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
                         for (int e = 0; e < VEC; ++e) ds[e] += r.get(e);
                     }
                     Vec<T, VEC> o;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) o.set(e, t < len ? ds[e] : 0.f);
-                    o.store_n(dxp + static_cast<long long>(t) * p.a.dim, n, p.vec_dx);
+                    o.put(ds);
+                    if (t >= len) o.zero();
+                    store_step<FULL>(o, dxp, n, p.vec_dx);
                 }
             }
 #pragma unroll
@@ -420,6 +444,7 @@ void conv_flags(ConvP& p) {
     p.vec_dy = d && vec_ok<T, VEC>(a.dy, a.dy_batch, a.dy_time);
     p.vec_dx = d && vec_ok<T, VEC>(a.dx, ds, 0);
     p.vec_dso = d && vec_ok<T, VEC>(a.dstate_out, ds, 0);
+    p.full = p.vec_x && p.vec_y && p.vec_dy && p.vec_dx;
 }
 
 template <typename T, bool BWD>
@@ -434,10 +459,17 @@ cudaError_t run_conv(const sdtw_conv_args& a, cudaStream_t st) {
         conv_geometry(p, VEC);
         conv_flags<T, VEC>(p);
         const unsigned g = static_cast<unsigned>(static_cast<long long>(p.nchb) * p.ntb * a.batch);
-        if constexpr (BWD)
-            conv_bwd_kernel<T, VEC, WT><<<g, kThreads, 0, st>>>(p);
-        else
-            conv_fwd_kernel<T, VEC, WT><<<g, kThreads, 0, st>>>(p);
+        if constexpr (BWD) {
+            if (p.full)
+                conv_bwd_kernel<T, VEC, WT, true><<<g, kThreads, 0, st>>>(p);
+            else
+                conv_bwd_kernel<T, VEC, WT, false><<<g, kThreads, 0, st>>>(p);
+        } else {
+            if (p.full)
+                conv_fwd_kernel<T, VEC, WT, true><<<g, kThreads, 0, st>>>(p);
+            else
+                conv_fwd_kernel<T, VEC, WT, false><<<g, kThreads, 0, st>>>(p);
+        }
     };
     if (a.width == 2) go(std::integral_constant<int, 2>{});
     else if (a.width == 3) go(std::integral_constant<int, 3>{});

@@ -96,11 +96,11 @@ struct LnWeights {
 __host__ __device__ constexpr int ln_threads(int tpr) { return tpr > 128 ? tpr : 128; }
 // Resident blocks to ask the compiler for: registers are the row's elements as
 // loaded (the next row's, and in the backward the present one's too) and the
-// float values in work (forward) or column sums (backward), and about 40 more.
+// float values in work (forward) or column sums (backward), and about 40 (56) more.
 // Single 16-bit elements take a register each.
 __host__ __device__ constexpr int ln_blocks(int elems, int vec, int esize, int threads, bool bwd) {
     const int raw = vec == 1 ? elems : elems * esize / 4;
-    const int regs = (bwd ? 2 * elems + 4 * raw : elems + raw) + 40;
+    const int regs = bwd ? 2 * elems + 4 * raw + 56 : elems + raw + 40;
     const int n = 65536 / (threads * (regs > 250 ? 250 : regs));
     return n < 1 ? 1 : (n > 8 ? 8 : n);
 }
@@ -143,13 +143,15 @@ __global__ void __launch_bounds__(ln_threads(TPR), ln_blocks(VEC* NV, VEC, sizeo
         const float mean = row_sum<TPR>(s, buf, turn) * inv;
         s = 0.f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            const bool in = (k * TPR + tid) * VEC < p.dim;  // all VEC of them: VEC divides dim
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 float& u = v[k * VEC + e];
-                u = (k * TPR + tid) * VEC + e < p.dim ? u - mean : 0.f;
+                u = in ? u - mean : 0.f;
                 s = fmaf(u, u, s);
             }
+        }
         const float rstd = rsqrtf(row_sum<TPR>(s, buf, turn) * inv + p.eps);
         T* yr = static_cast<T*>(p.y) + r * p.dim;
 #pragma unroll
@@ -160,7 +162,8 @@ __global__ void __launch_bounds__(ln_threads(TPR), ln_blocks(VEC* NV, VEC, sizeo
             bt.get(k, tid, b);
             Vec<T, VEC> o;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) o.set(e, fmaf(v[k * VEC + e] * rstd, w[e], b[e]));
+            for (int e = 0; e < VEC; ++e) w[e] = fmaf(v[k * VEC + e] * rstd, w[e], b[e]);
+            o.put(w);
             if (c < p.dim) o.store(yr + c);
         }
         if (tid == 0 && p.mean) {
@@ -241,8 +244,9 @@ __global__ void __launch_bounds__(ln_threads(TPR), ln_blocks(VEC* NV, VEC, sizeo
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float xh = (rx[k].get(e) - mean) * rs;
-                o.set(e, rs * (rg[k].get(e) * w[e] - s1 - xh * s2));
+                w[e] = rs * (rg[k].get(e) * w[e] - s1 - xh * s2);
             }
+            o.put(w);
             if (c < p.dim) o.store(dr + c);
         }
     }

@@ -105,8 +105,7 @@ __device__ __forceinline__ void st_store(const St& s, float* tab, long long row,
     float v[4];
     upk(s.v[0], v[0], v[1]);
     upk(s.v[1], v[2], v[3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.set(j, v[j]);
+    r.put(v);
     r.store_n(tab + row * S + n0, n, vec);
 }
 // h <- exp(A sum dt) h + E over one segment.

@@ -52,8 +52,8 @@ struct BwdSmem {
     float acc[2][kScanWarps][kTS][2][K::NP];  // the warps' dB, dC
 };
 
-template <typename T, int NL, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p) {
+template <typename T, int NL, bool FULL, int BLOCKS>
+__global__ void __launch_bounds__(kScanThreads, BLOCKS) scan_bwd_kernel(const ScanP p) {
     using K = ScanTile<NL>;
     using M = BwdSmem<T, NL>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -335,10 +335,13 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_bwd_kernel(const ScanP p
                 const float dd = fmaf(q[e], x[e], kLn2 * sr[e]) * ds[e];
                 dbias[e] += dd;
                 dD[e] = fmaf(g[e], x[e], dD[e]);
-                ox.set(e, fmaf(q[e], u[2 * e], g[e] * skip[e]));
-                od.set(e, dd);
-                oz.set(e, zf[e] * fmaf(skip[e], x[e], y[e]));
+                ds[e] = dd;
+                y[e] = zf[e] * fmaf(skip[e], x[e], y[e]);
+                q[e] = fmaf(q[e], u[2 * e], g[e] * skip[e]);
             }
+            ox.put(q);
+            od.put(ds);
+            oz.put(y);
             const int no = t < at.t1 ? nx : 0;
             const long long o = out0 + static_cast<long long>(t) * dim;
             if (p.a.dx) stage_store<FULL>(ox, static_cast<T*>(p.a.dx) + o, no, p.vec_dx);
@@ -445,7 +448,12 @@ cudaError_t run_scan_bwd(const sdtw_scan_args& a, cudaStream_t st) {
     const long long npar = (static_cast<long long>(a.dim) * (a.nstate + 2) + 255) / 256;
     if (blocks > 0x7fffffffll || nbc + npar > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     const int smem = static_cast<int>(sizeof(BwdSmem<T, NL>));
-    const auto kernel = p.full ? scan_bwd_kernel<T, NL, true> : scan_bwd_kernel<T, NL, false>;
+    // 168 registers a thread and three blocks per SM, or 128 (some spilled) and
+    // four, where that saves a round of blocks: measured at 512 blocks (32 x 512
+    // x 512) 298 against 248 us, at 384 (8 x 2048 x 1536) 729 against 780.
+    const long long rounds3 = (blocks + 148 * 3 - 1) / (148 * 3), rounds4 = (blocks + 148 * 4 - 1) / (148 * 4);
+    const auto kernel = !p.full ? scan_bwd_kernel<T, NL, false, 3>
+                                : (rounds4 < rounds3 && rounds3 <= 4 ? scan_bwd_kernel<T, NL, true, 4> : scan_bwd_kernel<T, NL, true, 3>);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (p.nseg > 1 && (e = launch_scan_segments(p, true, st)) != cudaSuccess) return e;

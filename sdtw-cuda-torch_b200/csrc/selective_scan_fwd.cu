@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanP p
                 const float z = rz.get(e);
                 y[e] *= z * sigmoidf(z);
             }
-            o.set(e, in ? y[e] : 0.f);
+            y[e] = in ? y[e] : 0.f;
         }
+        o.put(y);
         stage_store<FULL>(o, yp, t < at.t1 ? nx : 0, p.vec_y);
         yp += static_cast<long long>(kTS) * dim;
         __syncwarp();  // before the next piece but one comes into this one's place
@@ -245,23 +246,23 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const ScanP p) {
         b = static_cast<int>(i / p.a.dim);
         f = static_cast<int>(i % p.a.dim);
         const int g = f / p.dg, n = min(max(S - n0, 0), 4);
-        Vec<float, 4> A, h;
+        Vec<float, 4> A, out;
         A.load_n(p.a.A + static_cast<long long>(f) * S + n0, n, p.vec_n);
         // Plain loads: state_out may be the same tensor.
         const float* hp = p.a.state_in + b * p.a.state_in_batch + static_cast<long long>(f) * S + n0;
-        h.zero();
+        float h[4] = {};
         if (p.vec_n) {
             if (n > 0) {
                 const float4 q = *reinterpret_cast<const float4*>(hp);
-                h.set(0, q.x);
-                h.set(1, q.y);
-                h.set(2, q.z);
-                h.set(3, q.w);
+                h[0] = q.x;
+                h[1] = q.y;
+                h[2] = q.z;
+                h[3] = q.w;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (j < n) h.set(j, hp[j]);
+                if (j < n) h[j] = hp[j];
         }
         x = to_f(static_cast<const T*>(p.a.x)[b * p.a.x_batch + f]);
         float dt = to_f(static_cast<const T*>(p.a.delta)[b * p.a.delta_batch + f]);
@@ -272,10 +273,11 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const ScanP p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < n) {
-                h.set(j, fmaf(ex2f(dt * (A.get(j) * kL2e)), h.get(j), dt * x * to_f(Bp[j])));
-                y = fmaf(to_f(Cp[j]), h.get(j), y);
+                h[j] = fmaf(ex2f(dt * (A.get(j) * kL2e)), h[j], dt * x * to_f(Bp[j]));
+                y = fmaf(to_f(Cp[j]), h[j], y);
             }
-        h.store_n(p.a.state_out + b * p.a.state_out_batch + static_cast<long long>(f) * S + n0, n, p.vec_n);
+        out.put(h);
+        out.store_n(p.a.state_out + b * p.a.state_out_batch + static_cast<long long>(f) * S + n0, n, p.vec_n);
     }
 #pragma unroll
     for (int m = 1; m < NL; m *= 2) y += __shfl_xor_sync(0xffffffffu, y, m);

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstring>
 
 #include "sdtw_device.cuh"
 
@@ -37,6 +38,24 @@ __device__ __forceinline__ float half_bits<__nv_bfloat16>(uint32_t h) { return _
 __device__ __forceinline__ uint32_t bits_of(__half v) { return __half_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 
+// Two floats as 16-bit elements, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_bits(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pair_bits<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    uint32_t r;
+    memcpy(&r, &v, 4);
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pair_bits<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    uint32_t r;
+    memcpy(&r, &v, 4);
+    return r;
+}
+
 // V elements in 32-bit words, moved in pieces of at most 16 bytes.  16-bit
 // elements are loaded as unsigned short: the headers' __ldg of __half and
 // __nv_bfloat16 is an asm statement without `volatile`, which the compiler may
@@ -56,14 +75,18 @@ struct Vec {
         else
             return half_bits<T>(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
     }
-    // Elements must be set in order: an even one clears its word.
-    __device__ __forceinline__ void set(int e, float v) {
-        if constexpr (k32)
-            w[e] = __float_as_uint(v);
-        else if (e & 1)
-            w[e / 2] |= bits_of(from_f<T>(v)) << 16;
-        else
-            w[e / 2] = bits_of(from_f<T>(v));
+    // Rounds V floats.  Pairs at a time: a pair's conversion is one instruction
+    // of the ALU, a single one's takes the unit of the exponentials.
+    __device__ __forceinline__ void put(const float (&v)[V]) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (k32)
+                w[i] = __float_as_uint(v[i]);
+            else if constexpr (V == 1)
+                w[i] = bits_of(from_f<T>(v[0]));
+            else
+                w[i] = pair_bits<T>(v[2 * i], v[2 * i + 1]);
+        }
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
