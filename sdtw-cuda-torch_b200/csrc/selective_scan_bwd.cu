@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kScanThreads, BLOCKS) scan_bwd_kernel(const Sc
                 const St b = quad(&sm.B[buf][perm][sb + s][n0]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const f2 d = ex22(mul2(pk(du.x, du.x), A2.v[j]));
+                    const f2 d = decay(du.x, A2.v[j]);
                     s0.v[j] = fma2(d, s0.v[j], mul2(pk(du.y, du.y), b.v[j]));
                     if (keep) {
                         a[s][j] = d;

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanP p
                 const St b = quad(&st.B[sb + s][n0]), c = quad(&st.C[sb + s][n0]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j]));
+                    const f2 a = decay(du.x, A2.v[j]);
                     h.v[j] = fma2(a, h.v[j], mul2(pk(du.y, du.y), b.v[j]));
                 }
                 v[s] = sum2(fma2(c.v[1], h.v[1], mul2(c.v[0], h.v[0])));
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_segment_kernel(const ScanP 
             sum += du.x;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const f2 a = ex22(mul2(pk(du.x, du.x), A2.v[j])), u2 = pk(du.y, du.y);
+                const f2 a = decay(du.x, A2.v[j]), u2 = pk(du.y, du.y);
                 h.v[j] = REV ? mul2(a, fma2(u2, b.v[j], h.v[j])) : fma2(a, h.v[j], mul2(u2, b.v[j]));
             }
         }
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const ScanP p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < n) {
-                h[j] = fmaf(ex2f(dt * (A.get(j) * kL2e)), h[j], dt * x * to_f(Bp[j]));
+                h[j] = fmaf(ex2f(fmaf(dt, A.get(j) * kL2e, kExpLift)), h[j], dt * x * to_f(Bp[j]));
                 y = fmaf(to_f(Cp[j]), h[j], y);
             }
         out.put(h);
