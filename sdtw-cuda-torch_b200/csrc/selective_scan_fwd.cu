@@ -40,6 +40,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanP p
     const int row = lane / K::LR, col = lane % K::LR * K::VX;
     const int nx = FULL ? K::VX : min(max(at.nc - col, 0), K::VX);
     const bool vn = FULL || p.vec_n;
+    unsigned long long real[2];  // all bits of the states that exist
+#pragma unroll
+    for (int j = 0; j < 2; ++j) real[j] = (2 * j < ns ? 0xffffffffull : 0) | (2 * j + 1 < ns ? 0xffffffff00000000ull : 0);
 
     St A2 = st_load(p.a.A, f, S, n0, ns, vn), h;
     st_scale(A2, kL2e);
@@ -114,7 +117,13 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_fwd_kernel(const ScanP p
                     const f2 a = decay(du.x, A2.v[j]);
                     h.v[j] = fma2(a, h.v[j], mul2(pk(du.y, du.y), b.v[j]));
                 }
-                v[s] = sum2(fma2(c.v[1], h.v[1], mul2(c.v[0], h.v[0])));
+                if constexpr (FULL) {
+                    v[s] = sum2(fma2(c.v[1], h.v[1], mul2(c.v[0], h.v[0])));
+                } else {
+                    // States that do not exist are 0 while the step is finite; an infinite
+                    // one must not bring their 0 x infinity into the sum.
+                    v[s] = sum2(fma2(c.v[1], f2{h.v[1].v & real[1]}, mul2(c.v[0], f2{h.v[0].v & real[0]})));
+                }
             }
             using Sum = LaneSum<kRun, 1, NL>;
             Sum::run(v, lane);

@@ -206,7 +206,8 @@ __device__ __forceinline__ float dsilu(float v) {
 //          P of degree 5 fitted at Chebyshev nodes (1e-10); no small difference
 //          of near-equal numbers, so tiny step sizes keep their relative accuracy
 __device__ __forceinline__ float softplusf(float v, float* deriv = nullptr) {
-    const float n = -fabsf(v);
+    float n;  // -|v|, not below -126 (where e is 0 anyway), so that an infinite v gives no inf - inf; NaN stays
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(n) : "f"(-fabsf(v)), "f"(-126.f));
     const float t = n * 1.44269502f;
     const float lost = fmaf(n, 1.92596303e-8f, fmaf(n, 1.44269502f, -t));
     float e = ex2f(t);

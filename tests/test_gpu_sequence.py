@@ -246,6 +246,29 @@ def test_strong_decays_and_large_steps():
     assert torch.equal(y, torch.zeros_like(y))
 
 
+def test_infinite_and_nan_steps_follow_the_formula():
+    """delta of any size through softplus: 0 and the identity at the ends, NaN only from NaN."""
+    v = torch.tensor([float("inf"), 3e38, 1e30, 200.0, 88.0, 17.0, 1e-3, -17.0, -88.0, -200.0, -3e38, float("-inf"), float("nan")],
+                     device="cuda").reshape(-1, 1, 1)
+    one = torch.ones_like(v)
+    y = S.selective_scan(one, v, -torch.ones(1, 1, device="cuda"), one, one, delta_softplus=True)
+    want = torch.nn.functional.softplus(v.double(), threshold=1e4).float()
+    torch.testing.assert_close(y, want, rtol=1e-6, atol=1e-37, equal_nan=True)
+
+
+def test_steps_of_size_zero_keep_the_state_exactly():
+    rn = _gen(32)
+    h0 = rn(2, 8, 16)
+    x = rn(2, 100, 8)
+    bc = rn(2, 100, 16)
+    A = -torch.rand(8, 16, device="cuda") * 20
+    _, h = S.selective_scan(x, torch.zeros_like(x), A, bc, bc, initial_state=h0, return_state=True)
+    assert torch.equal(h, h0)
+    n = torch.zeros(2, dtype=torch.int64, device="cuda")
+    _, h = S.selective_scan(x, x, A, bc, bc, initial_state=h0, lengths=n, return_state=True)
+    assert torch.equal(h, h0)
+
+
 # ----------------------------------------------------------------------------- single steps, continued series
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("Bt,Dm,St,G,W", [(1, 1, 1, None, 1), (3, 33, 16, None, 4), (2, 30, 5, 3, 2), (5, 24, 64, 2, 8), (70, 64, 17, None, 3)])
@@ -274,6 +297,16 @@ def test_steps(dtype, Bt, Dm, St, G, W):
     version = past._version
     assert torch.equal(S.causal_conv_step(x[:, 0], w, b, state=past, activation="silu"), y)
     assert torch.equal(past, new) and past._version > version
+
+
+def test_steps_in_inference_mode():
+    with torch.inference_mode():
+        x, st = torch.ones(2, 8, device="cuda"), torch.zeros(2, 3, 8, device="cuda")
+        S.causal_conv_step(x, torch.ones(8, 4, device="cuda"), state=st)
+        assert torch.equal(st[:, -1], x)
+        h = torch.zeros(2, 8, 4, device="cuda")
+        S.selective_scan_step(x, x, -torch.ones(8, 4, device="cuda"), x[:, :4], x[:, :4], state=h)
+        assert (h == 1).all()
 
 
 def test_prompt_in_pieces_then_steps_is_one_series():
