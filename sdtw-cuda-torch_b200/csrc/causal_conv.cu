@@ -15,6 +15,7 @@
 // keeps the thread's dw and dbias in registers; the blocks' partial sums are
 // added by a second kernel in a fixed order.
 #include <algorithm>
+#include <cmath>
 
 #include "seq_device.cuh"
 #include "seq_kernels.h"
@@ -36,12 +37,22 @@ struct ConvP {
     float* part;
 };
 
-// Tile length: long tiles re-read less; shorter ones when there would be too
-// few threads to fill the GPU (148 SMs x 1024).
+// Tile length, a multiple of 16: long tiles re-read less, but the blocks should
+// come in whole rounds of the GPU (about 4 of 128 threads per SM are resident).
+// The length with the least rounds x (length + 8 steps' worth of start-up).
 int conv_tile(int batch, int length, int nch) {
-    int tt = 64;
-    while (tt > 16 && static_cast<long long>(batch) * ((length + tt - 1) / tt) * nch < 148ll * 1024) tt /= 2;
-    return tt;
+    int best = 16;
+    double cost = 1e300;
+    for (int tt = 16; tt <= 256; tt += 16) {
+        const double blocks = static_cast<double>(batch) * ((length + tt - 1) / tt) * nch / kThreads;
+        const double c = std::ceil(blocks / (148 * 4)) * (tt + 8);
+        if (c < cost) {
+            cost = c;
+            best = tt;
+        }
+        if (tt >= length) break;
+    }
+    return best;
 }
 // Features per thread: 4 (8 or 16 bytes a load); 2 for a width that is not 2, 3
 // or 4, whose arrays of kConvMaxWidth taps would not fit in registers.
@@ -142,7 +153,7 @@ __device__ __forceinline__ void store_step(const Vec<T, VEC>& r, T* q, int n, bo
 }
 
 template <typename T, int VEC, int WT, bool FULL>
-__global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
+__global__ void __launch_bounds__(kThreads, WT != 0 ? 4 : 3) conv_fwd_kernel(const ConvP p) {
     constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 8;
     const int W = Width<WT>::get(p.a.width);
     const ConvPlace<VEC> at(p);
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvP p) {
 }
 
 template <typename T, int VEC, int WT, bool FULL>
-__global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
+__global__ void __launch_bounds__(kThreads, WT != 0 && sizeof(T) == 2 ? 4 : 3) conv_bwd_kernel(const ConvP p) {
     constexpr int KM = Width<WT>::kMax, VP = VEC / 2, U = 4;
     const int W = Width<WT>::get(p.a.width);
     const ConvPlace<VEC> at(p);
@@ -259,60 +270,68 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvP p) {
                 to_pairs<T, VEC>(ng[u], gs[KM - 1 + u]);
             }
             if (j0 + U < j_end) fetch(j0 + U);
+            // Inside the tile and the valid steps no step needs a condition.
+            auto steps = [&](auto tag) {
+                constexpr bool inner = decltype(tag)::value;
 #pragma unroll
-            for (int u = 0; u < U; ++u, dxp += dt) {
-                const int j = j0 + u, t = j - (W - 1);
-                if (p.a.silu) {  // gv = dy times the derivative; dy is 0 from the valid steps' end on
+                for (int u = 0; u < U; ++u, dxp += dt) {
+                    const int j = j0 + u, t = j - (W - 1);
+                    if (p.a.silu) {  // gv = dy times the derivative; dy is 0 from the valid steps' end on
 #pragma unroll
-                    for (int q = 0; q < VP; ++q) {
-                        f2 v = k.bias[q];
+                        for (int q = 0; q < VP; ++q) {
+                            f2 v = k.bias[q];
 #pragma unroll
-                        for (int m = 0; m < KM; ++m)
-                            if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
-                        float a, b;
-                        upk(v, a, b);
-                        gs[KM - 1 + u][q] = mul2(gs[KM - 1 + u][q], pk(dsilu(a), dsilu(b)));
-                    }
-                }
-                if (j < t1) {
-#pragma unroll
-                    for (int q = 0; q < VP; ++q) {
-                        db[q] = add2(db[q], gs[KM - 1 + u][q]);
-#pragma unroll
-                        for (int m = 0; m < KM; ++m)
-                            if (m < W) dw[m][q] = fma2(gs[KM - 1 + u][q], xs[KM - 1 + u - m][q], dw[m][q]);
-                    }
-                }
-                if (p.a.dx && t >= t0 && t < t1) {
-                    float ds[VEC];
-#pragma unroll
-                    for (int q = 0; q < VP; ++q) {  // sum_k w[k] gv[j - k], w[k] = wr[W - 1 - k]
-                        f2 d = pk(0.f, 0.f);
-                        if constexpr (WT != 0) {
-#pragma unroll
-                            for (int i = 0; i < KM; ++i) d = fma2(k.wr[KM - 1 - i][q], gs[KM - 1 + u - i][q], d);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < KM; ++i)
-#pragma unroll
-                                for (int m = 0; m < KM; ++m)
-                                    if (m + i == W - 1) d = fma2(k.wr[m][q], gs[KM - 1 + u - i][q], d);
+                            for (int m = 0; m < KM; ++m)
+                                if (m < W) v = fma2(k.wr[m][q], xs[KM - 1 + u - m][q], v);
+                            float a, b;
+                            upk(v, a, b);
+                            gs[KM - 1 + u][q] = mul2(gs[KM - 1 + u][q], pk(dsilu(a), dsilu(b)));
                         }
-                        upk(d, ds[2 * q], ds[2 * q + 1]);
                     }
-                    if (p.a.dstate_out && t < len && j >= len) {
-                        Vec<T, VEC> r;
-                        r.load_n(static_cast<const T*>(p.a.dstate_out) + (static_cast<long long>(at.b) * (W - 1) + (j - len)) * p.a.dim + c, n,
-                                 p.vec_dso);
+                    if (inner || j < t1) {
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) ds[e] += r.get(e);
+                        for (int q = 0; q < VP; ++q) {
+                            db[q] = add2(db[q], gs[KM - 1 + u][q]);
+#pragma unroll
+                            for (int m = 0; m < KM; ++m)
+                                if (m < W) dw[m][q] = fma2(gs[KM - 1 + u][q], xs[KM - 1 + u - m][q], dw[m][q]);
+                        }
                     }
-                    Vec<T, VEC> o;
-                    o.put(ds);
-                    if (t >= len) o.zero();
-                    store_step<FULL>(o, dxp, n, p.vec_dx);
+                    if (inner || (p.a.dx && t >= t0 && t < t1)) {
+                        float ds[VEC];
+#pragma unroll
+                        for (int q = 0; q < VP; ++q) {  // sum_k w[k] gv[j - k], w[k] = wr[W - 1 - k]
+                            f2 d = pk(0.f, 0.f);
+                            if constexpr (WT != 0) {
+#pragma unroll
+                                for (int i = 0; i < KM; ++i) d = fma2(k.wr[KM - 1 - i][q], gs[KM - 1 + u - i][q], d);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < KM; ++i)
+#pragma unroll
+                                    for (int m = 0; m < KM; ++m)
+                                        if (m + i == W - 1) d = fma2(k.wr[m][q], gs[KM - 1 + u - i][q], d);
+                            }
+                            upk(d, ds[2 * q], ds[2 * q + 1]);
+                        }
+                        if (!inner && p.a.dstate_out && t < len && j >= len) {
+                            Vec<T, VEC> r;
+                            r.load_n(static_cast<const T*>(p.a.dstate_out) + (static_cast<long long>(at.b) * (W - 1) + (j - len)) * p.a.dim + c, n,
+                                     p.vec_dso);
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) ds[e] += r.get(e);
+                        }
+                        Vec<T, VEC> o;
+                        o.put(ds);
+                        if (!inner && t >= len) o.zero();
+                        store_step<FULL>(o, dxp, n, p.vec_dx);
+                    }
                 }
-            }
+            };
+            if (p.a.dx && j0 >= t0 + W - 1 && j0 + U <= min(t1, len))
+                steps(std::true_type{});
+            else
+                steps(std::false_type{});
 #pragma unroll
             for (int m = 0; m < KM - 1; ++m)
 #pragma unroll
