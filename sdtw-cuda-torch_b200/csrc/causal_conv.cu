@@ -13,7 +13,10 @@
 // before the present ones are worked on, and the multiply-adds are packed pairs
 // of features.  The backward computes v again from x instead of storing it, and
 // keeps the thread's dw and dbias in registers; the blocks' partial sums are
-// added by a second kernel in a fixed order.
+// added by a second kernel in a fixed order.  Measured on B200 at 16 x 2048 x 1536
+// bfloat16, width 4, with v sigmoid(v): 49 us forward (4.1 TB/s), 89 us backward
+// (3.4 TB/s).  Both issue an instruction every other cycle of their schedulers;
+// two uses of the exponentials' unit per element take 22 us of it.
 #include <algorithm>
 #include <cmath>
 
