@@ -189,6 +189,18 @@ def test_selective_scan(Bt, N, Dm, St, G, dtype, opts, ragged, state):
     _check_scan(c, n, h0, dy, dh, opts, state)
 
 
+@pytest.mark.parametrize("Bt,N,Dm,St,G", [
+    (2, 37, 64, 4, 2),      # whole tiles of 32 features
+    (1, 50, 24, 32, 3),     # of 4
+    (500, 18, 32, 16, 1),   # more blocks than three per SM: the variant with four
+    (1, 1000, 32, 16, 1),   # few warps: segments of time, whole tiles
+    (2, 900, 7, 5, 1)])     # the same with ragged ones
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_selective_scan_variants(Bt, N, Dm, St, G, dtype):
+    c, n, h0, dy, dh = _scan_case(N + Dm, Bt, N, Dm, St, G, dtype, Bt > 1, True)
+    _check_scan(c, n, h0, dy, dh, True, True)
+
+
 def test_selective_scan_long():
     c, n, h0, dy, dh = _scan_case(3, 2, 700, 24, 16, None, torch.float32, True, True)
     _check_scan(c, n, h0, dy, dh, True, True)
