@@ -43,9 +43,9 @@ constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // and -1 (measured; the error itself is up to 2 times 2^-24).  A state remembers
 // 1 / (dt |A|) steps, over which the average adds up: without a correction dA was
 // twice as far from float64 as with correctly rounded decays.  The exponents are
-// therefore raised by 0.2 x 2^-24 / ln 2, in the multiplication that makes them;
+// therefore raised by 0.3 x 2^-24 / ln 2, in the multiplication that makes them;
 // 2^(this) alone is still exactly 1, so a step of size 0 leaves the state as it is.
-constexpr float kExpLift = 1.72e-8f;
+constexpr float kExpLift = 2.58e-8f;
 
 template <int NL>
 struct ScanTile {
