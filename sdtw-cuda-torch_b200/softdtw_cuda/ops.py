@@ -281,7 +281,8 @@ def _(x, delta, A, B, C, D, z, delta_bias, softplus, lengths, initial_state, wan
     Bt, N, Dm = x.shape
     S, f32 = A.shape[1], torch.float32
     return (x.new_empty(x.shape), x.new_empty((Bt, Dm, S) if want_state else _EMPTY, dtype=f32),
-            x.new_empty((_native.scan_saved_elems(Bt, N, Dm, S),) if save else _EMPTY, dtype=f32))
+            # sdtw_scan_saved_elems, written out: the sizes may be symbolic here.
+            x.new_empty((Bt * ((N + 15) // 16) * Dm * S,) if save else _EMPTY, dtype=f32))
 
 
 @torch.library.custom_op("softdtw_cuda::selective_scan_backward", mutates_args=(), device_types="cuda")

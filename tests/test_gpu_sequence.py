@@ -506,6 +506,17 @@ def test_compiled_block_matches_eager(backend):
         assert torch.equal(step(xt, st2), want) and torch.equal(st, st2)
 
 
+def test_compiled_block_with_changing_lengths():
+    p = _block_params()
+    f = lambda x: _block(p, x).square().sum()  # noqa: E731
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    for N in (33, 40, 47, 5):
+        x = _gen(N)(2, N, 16).requires_grad_(True)
+        want = torch.autograd.grad(f(x), [x, *p.values()])
+        for a, b in zip(torch.autograd.grad(compiled(x), [x, *p.values()]), want):
+            torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
+
+
 def test_opcheck():
     rn = _gen(83)
     x, w, b = rn(2, 9, 6).requires_grad_(True), rn(6).requires_grad_(True), rn(6).requires_grad_(True)
